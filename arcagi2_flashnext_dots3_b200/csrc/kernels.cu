@@ -17,6 +17,7 @@ void register_dsa(pybind11::module& m);
 void register_f8gemm(pybind11::module& m);
 void register_moe_i8(pybind11::module& m);
 void register_gdn_chunk(pybind11::module& m);
+void register_vocab(pybind11::module& m);
 
 void register_kernels(pybind11::module& m) {
   register_fn(m);
@@ -32,4 +33,5 @@ void register_kernels(pybind11::module& m) {
   register_f8gemm(m);
   register_moe_i8(m);
   register_gdn_chunk(m);
+  register_vocab(m);
 }

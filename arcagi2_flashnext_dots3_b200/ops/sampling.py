@@ -210,3 +210,83 @@ def speculative_accept(logits: torch.Tensor, drafts: torch.Tensor, temps, seeds,
         acc.append(a)
         nxt.append(t)
     return acc, nxt
+
+
+def speculative_verify(logits: torch.Tensor, drafts: torch.Tensor, temps: torch.Tensor, seeds: torch.Tensor,
+                       steps: torch.Tensor, draft_logits: torch.Tensor = None, n_draft: torch.Tensor = None):
+    """:func:`speculative_accept` for whole batches on the device (csrc/k_vocab.cu), with nothing read by the host:
+    logits [B, k + 1, V] (fp32, fp16 or bf16; rows may be strided), drafts [B, k] int32 / int64, temps fp32 [B],
+    seeds and steps int64 [B]. Returns (accepted [B], next token [B]) int32 tensors.
+
+    ``draft_logits`` [B, k, V]: the distributions the drafts were drawn from, q = softmax(draft_logits / T). Draft j
+    is then accepted while u q_j(d) < p_j(d) and the first rejected position draws from max(p - q, 0), normalized;
+    without them a draft is a point mass, q(d) = 1. The drafts must come from another seed than the verification, whose
+    noise of (seed, step + j, token) they would otherwise share. ``n_draft`` int32 [B]: drafts of each sequence, 0 to
+    k; later positions are not read.
+
+    T <= 0 is greedy: accepted while the draft is the argmax (lowest id on ties), which is also the next token. A draft
+    outside the vocabulary is rejected. Masked logits (at or below -1e30) are never drawn; a residual that is empty in
+    fp32 draws from p; a position with no token left gives -1."""
+    if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
+        raise ValueError(f"logits: expected [B, k + 1, V], got {tuple(logits.shape)}")
+    B, k1, V = logits.shape
+    k = k1 - 1
+    if drafts.shape != (B, k) or drafts.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"drafts: expected int32 / int64 [{B}, {k}], got {drafts.dtype} {tuple(drafts.shape)}")
+    for name, t, ty in (("temps", temps, torch.float32), ("seeds", seeds, torch.int64), ("steps", steps, torch.int64),
+                        ("n_draft", n_draft, torch.int32)):
+        if t is not None and (t.shape != (B,) or t.dtype != ty):
+            raise ValueError(f"{name}: expected {ty} [{B}], got {t.dtype} {tuple(t.shape)}")
+    if draft_logits is not None and (draft_logits.shape != (B, k, V) or draft_logits.dtype != logits.dtype):
+        raise ValueError(f"draft_logits: expected {logits.dtype} [{B}, {k}, {V}], got {draft_logits.dtype} "
+                         f"{tuple(draft_logits.shape)}")
+    if logits.is_cuda:
+        accepted = torch.empty(B, dtype=torch.int32, device=logits.device)
+        nxt = torch.empty_like(accepted)
+        unit = lambda x: x if x is None or V == 1 or x.stride(2) == 1 else x.contiguous()  # noqa: E731
+        native.C().spec_verify(unit(logits.detach()), drafts.contiguous(), temps.contiguous(), seeds.contiguous(),
+                               steps.contiguous(), unit(draft_logits), None if n_draft is None else n_draft.contiguous(),
+                               accepted, nxt)
+        return accepted, nxt
+    got = [_verify_one(logits[b], drafts[b].tolist()[:k if n_draft is None else max(0, int(n_draft[b]))],
+                       float(temps[b]), int(seeds[b]), int(steps[b]),
+                       None if draft_logits is None else draft_logits[b]) for b in range(B)]
+    out = torch.tensor(got, dtype=torch.int32).view(B, 2)
+    return out[:, 0].contiguous(), out[:, 1].contiguous()
+
+
+def _probabilities(row: torch.Tensor, T: float) -> torch.Tensor:
+    z = row.float()
+    z = z.masked_fill(z <= -1e30, float("-inf")) / T
+    m = z.max()
+    return torch.zeros_like(z) if m == float("-inf") else torch.softmax(z, -1)
+
+
+def _verify_one(lg: torch.Tensor, drafts: list, T: float, seed: int, step: int, draft_lg=None):
+    """speculative_verify of one sequence: lg [k + 1, V], at most k drafts."""
+    V = lg.shape[-1]
+    idx = torch.arange(V, device=lg.device)
+    for j in range(len(drafts) + 1):
+        d = drafts[j] if j < len(drafts) else -1
+        if not T > 0:
+            z = lg[j].float()
+            best = int(z.argmax()) if bool((z > -1e30).any()) else -1
+            if d >= 0 and d == best:
+                continue
+            return j, best
+        p = _probabilities(lg[j], T)
+        r = p
+        if j < len(drafts):
+            q = None if draft_lg is None else _probabilities(draft_lg[j], T)
+            if 0 <= d < V:
+                u = float(uniform_torch(seed, step + j, torch.tensor([ACCEPT_INDEX]))[0])
+                if u * (1.0 if q is None else float(q[d])) < float(p[d]):
+                    continue
+            r = torch.where(idx == d, 0.0, p) if q is None else (p - q).clamp_min(0.0)
+            if not bool((r > 0).any()):
+                r = p
+        if not bool((r > 0).any()):
+            return j, -1
+        race = -torch.log(uniform_torch(seed, step + j, idx)) / r
+        return j, int(torch.where(r > 0, race, float("inf")).argmin())
+    raise AssertionError("the position after the last draft always returns")
