@@ -10,7 +10,7 @@ PKG = "arcagi2_flashnext_dots3_b200"
 CSRC = os.path.join(PKG, "csrc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
-cuda_sources = [os.path.join(CSRC, f) for f in ("ext.cpp", "wgemm.cu")] + sorted(
+cuda_sources = [os.path.join(CSRC, f) for f in ("ext.cpp", "vocab.cpp", "wgemm.cu")] + sorted(
     f for f in glob.glob(os.path.join(CSRC, "k_*.cu")))
 cuda_sources.append(os.path.join(CSRC, "kernels.cu"))
 
