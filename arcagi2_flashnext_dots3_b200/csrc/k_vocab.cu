@@ -24,19 +24,22 @@
 // no distribution: its losses and gradients are 0, its recorded ids -1, its next token -1. Sums, maxima and all
 // statistics are fp32 (the teacher's tail mass, a difference from 1, in fp64).
 //
-// Work split. Every operator reads its logits once and is bound by that stream (and the gradient's), so:
-//   * a row is cut into 16-byte vectors over the C blocks of a thread-block cluster, C chosen so that a block's slice
-//     fits a few times into an SM's shared memory and few rows still fill the GPU (see plan_of);
-//   * a slice is copied asynchronously (cp.async) into shared memory; a thread reads back only the vectors that it
-//     copied, so the statistics need no block barrier before them and a second pass over the row costs no memory
-//     traffic;
-//   * one pass takes the running maximum and sum of a softmax; the blocks of a cluster exchange their sums through
-//     distributed shared memory (each writes its part into every peer, one cluster barrier) and each finishes the row
-//     statistics by itself, in rank order: bits do not depend on timing;
+// Work split. Every operator is bound by reading its logits once (and writing the gradient once), so a row is cut into
+// units of a few 16-byte vectors per thread that spread over the whole GPU:
+//   * forms with one look at the logits (top-k, the loss alone, verification) take a unit per block, straight into
+//     registers; a second small kernel, started early, joins the units' parts of a row in order;
+//   * gradients from saved statistics are elementwise: a unit per block;
+//   * forms that look twice (loss with gradient, acceptance) give a row to one block per SM, or to a cluster of them when
+//     there are few rows. A block copies as much of its slice as fits into shared memory (cp.async, read back only by the
+//     thread that copied it) and streams the rest, once for each look: the second time it comes from L2, since 148 such
+//     remainders fit there. Nothing is exchanged outside a cluster, whose blocks write their parts into each other's shared
+//     memory and finish the row's statistics each by itself, in rank order;
 //   * exp(x) is ex2(x log2 e / T - c) with c = m log2 e / T rounded once and used for the sum and for every
 //     probability alike, so that rounding cancels; one FMA and one ex2 per element.
-#include <cfloat>
+#include <algorithm>
 #include <cstdint>
+#include <cstdlib>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "ptx.cuh"
@@ -48,7 +51,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kBatch = 8;            // vectors that a thread holds at once
 constexpr int kMaxCluster = 16;
+constexpr int kRowThreads = 256;     // of the kernels that look twice
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kRowBlocks = 5;       // their blocks per SM
+constexpr int kKeep = 2560;          // vectors of a block that shared memory keeps (40 KB)
 constexpr float kTailFloor = 1e-8f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -71,6 +79,7 @@ template <> struct Vec<float> {
   static __device__ __forceinline__ float back(float x) { return x; }
 };
 template <> struct Vec<__half> {
+  using Pair = __half2;
   static constexpr int N = 8;
   static constexpr uint32_t kPad = 0xFC00FC00u;
   static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
@@ -92,6 +101,7 @@ template <> struct Vec<__half> {
   static __device__ __forceinline__ __half back(float x) { return __float2half_rn(x); }
 };
 template <> struct Vec<__nv_bfloat16> {
+  using Pair = __nv_bfloat162;
   static constexpr int N = 8;
   static constexpr uint32_t kPad = 0xFF80FF80u;
   static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
@@ -119,6 +129,43 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 operations per instruction.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ Two two(float a) { return two(a, a); }
+__device__ __forceinline__ float2 halves(Two a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two ex2_two(Two a) {
+  const float2 f = halves(a);
+  return two(ex2(f.x), ex2(f.y));
+}
+__device__ __forceinline__ float sum(Two a) {
+  const float2 f = halves(a);
+  return f.x + f.y;
 }
 
 // ------------------------------------------------------------------------------------------- clusters
@@ -156,54 +203,158 @@ template <typename T>
 struct Slice {
   const T* row;
   int V, phase, first, count;
+  bool inside;                       // every vector lies whole in the row
   __device__ __forceinline__ Slice(const T* r, int V_, int per, uint32_t rank) : row(r), V(V_) {
     constexpr int N = Vec<T>::N;
     phase = (int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
     const int total = (V + phase + N - 1) / N;
     first = min((int)rank * per, total);
     count = min(per, total - first);
-  }
+    inside = start(0) >= 0 && start(per - 1) + N <= V;
+  }   // rank * per stays below 2^31: V is at most kMaxV
   __device__ __forceinline__ int start(int v) const { return (first + v) * Vec<T>::N - phase; }   // first element
   __device__ __forceinline__ bool full(int i0) const { return i0 >= 0 && i0 + Vec<T>::N <= V; }
-  // the shared-memory place of element i when this block owns it, else -1
+  // the place of element i in the slice, -1 when it is not in it
   __device__ __forceinline__ int place(int i) const {
     const int at = i + phase - first * Vec<T>::N;
     return at >= 0 && at < count * Vec<T>::N ? at : -1;
   }
 };
 
-// Starts the copy of this thread's vectors of elements laid out as in `s`, taken from `row` (the slice's own row or
-// another one); out-of-row lanes become -inf. Vectors that `row` does not hold at a 16-byte boundary (the ends of a
-// row, a second row with another phase) go through plain loads.
+// This thread's vectors of `row` at the places of slice `s` (of that row or another one) in registers, -inf where the row
+// has no element. Ends of rows, and rows that start on different 16-byte boundaries, go element by element.
 template <typename T>
-__device__ __forceinline__ void load_slice(const Slice<T>& s, const T* row, uint4* sm) {
+__device__ __forceinline__ uint4 ragged_vec(const Slice<T>& s, const T* row, int i0) {
   constexpr int N = Vec<T>::N;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(s.row)) & 15) == 0;
-  for (int v = threadIdx.x; v < s.count; v += kThreads) {
-    const int i0 = s.start(v);
-    if (aligned && s.full(i0)) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(sm + v)), "l"(row + i0) : "memory");
-    } else {
-      T* d = reinterpret_cast<T*>(sm + v);
-      const uint32_t pad = Vec<T>::kPad;
+  float f[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        d[k] = i0 + k >= 0 && i0 + k < s.V ? row[i0 + k] : *reinterpret_cast<const T*>(&pad);
+  for (int k = 0; k < N; ++k) f[k] = i0 + k >= 0 && i0 + k < s.V ? Vec<T>::one(row[i0 + k]) : -INFINITY;
+  return Vec<T>::pack(f);
+}
+template <typename T, int kVec>
+__device__ __forceinline__ void load_unit(const Slice<T>& s, const T* row, int first, uint4 (&x)[kVec]) {
+  const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(s.row)) & 15) == 0;
+  const int v = first + threadIdx.x;
+  if (same && s.inside) {
+    const uint4* p = reinterpret_cast<const uint4*>(row + s.start(v));
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) x[i] = __ldcs(p + i * kThreads);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int i0 = s.start(v + i * kThreads);
+    x[i] = same && s.full(i0) ? __ldcs(reinterpret_cast<const uint4*>(row + i0)) : ragged_vec(s, row, i0);
+  }
+}
+template <typename T, int kVec>
+__device__ __forceinline__ void load_unit(const Slice<T>& s, uint4 (&x)[kVec]) {
+  load_unit(s, s.row, 0, x);
+}
+// A block's share of a row in the kernels that look twice: `n` whole vectors from element `e0`, which lies on a 16-byte
+// boundary, and the elements in front of the row's first boundary and behind its last, which the first and the last block
+// of the cluster take one by one. `kept` of the vectors (whole rounds of the block) stay in shared memory.
+constexpr int kRound = 4 * kRowThreads;
+template <typename T>
+struct Share {
+  const T* row;
+  int e0, n, kept, head, tail0, tail;   // head: [0, head), tail: [tail0, tail0 + tail)
+  __device__ __forceinline__ Share(const T* r, int V, uint32_t rank, uint32_t size, int keep) : row(r) {
+    constexpr int N = Vec<T>::N;
+    const int phase = (int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
+    const int lead = min((N - phase) % N, V), all = (V - lead) / N, per = (all + size - 1) / size;
+    const int first = min((int)rank * per, all);
+    e0 = lead + first * N;
+    n = min(per, all - first);
+    kept = min(n, keep) / kRound * kRound;
+    head = rank == 0 ? lead : 0;
+    tail0 = lead + all * N;
+    tail = rank == size - 1 ? V - tail0 : 0;
+  }
+  // the single element of this thread, -1 where it has none
+  __device__ __forceinline__ int single() const {
+    const int t = threadIdx.x;
+    return t < head ? t : t >= 32 && t - 32 < tail ? tail0 + t - 32 : -1;
+  }
+  __device__ __forceinline__ bool holds(int id) const {
+    return (id >= e0 && id < e0 + n * Vec<T>::N) || id < head || (id >= tail0 && id < tail0 + tail);
+  }
+  // whether element id, held by the block, is in one of this thread's vectors
+  __device__ __forceinline__ bool owns(int id) const {
+    return id >= e0 && id < e0 + n * Vec<T>::N && (id - e0) / Vec<T>::N % kRowThreads == (int)threadIdx.x;
+  }
+};
+template <typename T>
+__device__ __forceinline__ bool same_phase(const T* a, const T* b) {
+  return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+}
+// Starts the copy of the kept vectors of `row` (the share's own or another one) to sm[v], by the thread that reads them.
+template <typename T>
+__device__ __forceinline__ void copy_kept(const Share<T>& s, const T* row, uint4* sm) {
+  const T* p = row + s.e0 + threadIdx.x * Vec<T>::N;
+  if (same_phase(row, s.row)) {
+    const uint32_t d = smem_u32(sm + threadIdx.x);
+    for (int v = 0; v < s.kept; v += kRound)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + (v + i * kRowThreads) * 16),
+                     "l"(p + (v + i * kRowThreads) * Vec<T>::N) : "memory");
+  } else {
+    for (int v = 0; v < s.kept; v += kRowThreads) {
+      T* d = reinterpret_cast<T*>(sm + v + threadIdx.x);
+#pragma unroll
+      for (int k = 0; k < Vec<T>::N; ++k) d[k] = p[v * Vec<T>::N + k];
     }
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
 }
-__device__ __forceinline__ void wait_slices() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
-
-// Stores a vector of results: whole when it lies inside the row on a 16-byte boundary of `out`, else by elements.
-template <typename T>
-__device__ __forceinline__ void store_vec(const Slice<T>& s, T* out, bool aligned, int i0, const float (&f)[Vec<T>::N]) {
-  if (aligned && s.full(i0)) {
-    *reinterpret_cast<uint4*>(out + i0) = Vec<T>::pack(f);
-  } else {
+// Vectors v, v + kRowThreads, .. of the share from memory; -inf past its end.
+template <typename T, int kVec>
+__device__ __forceinline__ void stream(const Share<T>& s, const T* row, bool same, int v, uint4 (&x)[kVec]) {
+  constexpr int N = Vec<T>::N;
+  const T* p = row + s.e0 + v * N;
+  if (same && v + (kVec - 1) * kRowThreads < s.n) {
 #pragma unroll
-    for (int k = 0; k < Vec<T>::N; ++k)
-      if (i0 + k >= 0 && i0 + k < s.V) out[i0 + k] = Vec<T>::back(f[k]);
+    for (int i = 0; i < kVec; ++i) x[i] = __ldcg(reinterpret_cast<const uint4*>(p) + i * kRowThreads);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    x[i] = make_uint4(Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad);
+    if (v + i * kRowThreads < s.n) {
+      if (same) {
+        x[i] = __ldcg(reinterpret_cast<const uint4*>(p) + i * kRowThreads);
+      } else {
+        T* e = reinterpret_cast<T*>(&x[i]);
+#pragma unroll
+        for (int k = 0; k < N; ++k) e[k] = p[i * kRowThreads * N + k];
+      }
+    }
+  }
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ void store_ragged(const Slice<T>& s, T* out, int i0, const uint4& u) {
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int k = 0; k < Vec<T>::N; ++k)
+    if (i0 + k >= 0 && i0 + k < s.V) out[i0 + k] = e[k];
+}
+// Stores this thread's vectors f(0), f(1), .. of a unit of results to `out`, laid out as slice `s`.
+template <int kVec, typename T, typename F>
+__device__ __forceinline__ void store_unit(const Slice<T>& s, T* out, F f) {
+  const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(s.row)) & 15) == 0;
+  if (same && s.inside) {
+    uint4* p = reinterpret_cast<uint4*>(out + s.start(threadIdx.x));
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) __stcs(p + i * kThreads, f(i));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int i0 = s.start(threadIdx.x + i * kThreads);
+    if (same && s.full(i0)) *reinterpret_cast<uint4*>(out + i0) = f(i);
+    else store_ragged(s, out, i0, f(i));
   }
 }
 
@@ -216,43 +367,37 @@ __device__ __forceinline__ Soft join(Soft a, Soft b) {
   const float c = fmaxf(a.c, b.c);
   return {c, a.sum * ex2(a.c - c) + b.sum * ex2(b.c - c)};
 }
+__device__ __forceinline__ Soft as_soft(unsigned long long u) {
+  return {__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32))};
+}
 __device__ __forceinline__ Soft shfl_xor(Soft a, int o) {
   return {__shfl_xor_sync(0xffffffffu, a.c, o), __shfl_xor_sync(0xffffffffu, a.sum, o)};
 }
 
-template <int N>
-__device__ __forceinline__ float vec_max(const float (&f)[N]) {
-  float m = fmaxf(f[0], f[1]);
-#pragma unroll
-  for (int k = 2; k < N; ++k) m = fmaxf(m, f[k]);
-  return m;
+// Extremes of a vector; 16-bit types take them in pairs.
+template <typename T>
+__device__ __forceinline__ float packed_max(const uint4& u) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else {
+    using T2 = typename Vec<T>::Pair;
+    const T2* p = reinterpret_cast<const T2*>(&u);
+    const T2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(Vec<T>::one(m.x), Vec<T>::one(m.y));
+  }
 }
-template <int N>
-__device__ __forceinline__ float vec_min(const float (&f)[N]) {
-  float m = fminf(f[0], f[1]);
-#pragma unroll
-  for (int k = 2; k < N; ++k) m = fminf(m, f[k]);
-  return m;
+template <typename T>
+__device__ __forceinline__ float packed_min(const uint4& u) {
+  if constexpr (sizeof(T) == 4) {
+    return fminf(fminf(__uint_as_float(u.x), __uint_as_float(u.y)), fminf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else {
+    using T2 = typename Vec<T>::Pair;
+    const T2* p = reinterpret_cast<const T2*>(&u);
+    const T2 m = __hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3]));
+    return fminf(Vec<T>::one(m.x), Vec<T>::one(m.y));
+  }
 }
 __device__ __forceinline__ float masked(float z) { return z < kFloor ? -INFINITY : z; }
-template <int N>
-__device__ __forceinline__ void add_soft(const float (&f)[N], float kl, float& m, Soft& s) {
-  const float vm = vec_max(f);
-  if (vm > m) {
-    m = vm;
-    const float c = vm * kl;
-    s.sum *= ex2(s.c - c);
-    s.c = c;
-  }
-  float a = 0.f, b = 0.f;
-#pragma unroll
-  for (int k = 0; k < N; k += 2) {
-    a += ex2(fmaf(f[k], kl, -s.c));
-    b += ex2(fmaf(f[k + 1], kl, -s.c));
-  }
-  s.sum += a + b;
-}
-
 template <typename V, typename Op>
 __device__ __forceinline__ V warp_reduce(V v, Op op) {
 #pragma unroll
@@ -279,27 +424,83 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
   return __uint_as_float((ord & 0x80000000u) ? (ord ^ 0x80000000u) : ~ord);
 }
 
-// The softmax of a whole row from the blocks' parts: block -> cluster. `warp_part` and `part` are this kernel's shared
-// scratch ([kWarps], [kMaxCluster]); ends behind a cluster barrier.
-__device__ __forceinline__ Soft row_soft(Soft s, uint32_t rank, uint32_t size, unsigned long long* warp_part,
-                                         unsigned long long* part) {
+// A warp's part of a unit: its threads share their offset, so it is one maximum and one sum. `m`: the thread's largest logit,
+// or kFloor.
+template <typename T, int kVec>
+__device__ __forceinline__ Soft warp_soft(const uint4 (&x)[kVec], float m, float kl) {
+  constexpr int N = Vec<T>::N;
+  const float c = warp_reduce(m, Max()) * kl;
+  const Two k2 = two(kl), c2 = two(-c);
+  Two a = two(0.f), b = two(0.f);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s = join(s, shfl_xor(s, o));
-  if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = as_u64(s.c, s.sum);
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    const unsigned long long w = warp_part[threadIdx.x & (kWarps - 1)];
-    s = {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))};
+  for (int i = 0; i < kVec; ++i) {
+    float f[N];
+    Vec<T>::unpack(x[i], f);
 #pragma unroll
-    for (int o = kWarps / 2; o; o >>= 1) s = join(s, shfl_xor(s, o));
-    if (threadIdx.x < size) st_peer(part + rank, threadIdx.x, as_u64(s.c, s.sum));
+    for (int k = 0; k < N; k += 4) {
+      a = add2(a, ex2_two(fma2(two(f[k], f[k + 1]), k2, c2)));
+      b = add2(b, ex2_two(fma2(two(f[k + 2], f[k + 3]), k2, c2)));
+    }
   }
-  cluster_sync();
-  Soft r{__uint_as_float((uint32_t)part[0]), __uint_as_float((uint32_t)(part[0] >> 32))};
-  for (uint32_t i = 1; i < size; ++i)
-    r = join(r, Soft{__uint_as_float((uint32_t)part[i]), __uint_as_float((uint32_t)(part[i] >> 32))});
-  return r;
+  return {c, warp_reduce(sum(add2(a, b)), Add())};
 }
+template <typename T, int kVec>
+__device__ __forceinline__ float unit_max(const uint4 (&x)[kVec]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = packed_max<T>(x[0]);
+#pragma unroll
+    for (int i = 1; i < kVec; ++i) m = fmaxf(m, packed_max<T>(x[i]));
+    return m;
+  } else {
+    using T2 = typename Vec<T>::Pair;
+    T2 m = *reinterpret_cast<const T2*>(&x[0]);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const T2* p = reinterpret_cast<const T2*>(&x[i]);
+      m = __hmax2(m, __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3])));
+    }
+    return fmaxf(Vec<T>::one(m.x), Vec<T>::one(m.y));
+  }
+}
+// Adds vectors to a thread's running softmax with maximum m.
+template <typename T, int kVec>
+__device__ __forceinline__ void add_soft(const uint4 (&x)[kVec], float kl, float& m, Soft& s) {
+  constexpr int N = Vec<T>::N;
+  const float vm = unit_max<T>(x);
+  if (vm > m) {
+    m = vm;
+    const float c = vm * kl;
+    s.sum *= ex2(s.c - c);
+    s.c = c;
+  }
+  const Two k2 = two(kl), c2 = two(-s.c);
+  Two a = two(0.f), b = two(0.f);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    float f[N];
+    Vec<T>::unpack(x[i], f);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      a = add2(a, ex2_two(fma2(two(f[k], f[k + 1]), k2, c2)));
+      b = add2(b, ex2_two(fma2(two(f[k + 2], f[k + 3]), k2, c2)));
+    }
+  }
+  s.sum += sum(add2(a, b));
+}
+// Joins a list of parts over a warp, in an order that depends on their number alone: every lane gets the same bits.
+template <typename Load>
+__device__ __forceinline__ Soft join_parts(int n, float kl, Load load) {
+  Soft t{kFloor * kl, 0.f};
+  for (int i = threadIdx.x & 31; i < n; i += 32) t = join(t, as_soft(load(i)));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) t = join(t, shfl_xor(t, o));
+  return t;
+}
+
+// Kernels that look once: block (x, y, z) takes unit x of row y + z gridDim.y (neighbouring blocks in neighbouring memory:
+// with the rows along x the gradients ran at 93% of the copy rate instead of 100%).
+__device__ __forceinline__ int64_t unit_row() { return (int64_t)blockIdx.z * gridDim.y + blockIdx.y; }
+__device__ __forceinline__ int64_t unit_index() { return unit_row() * gridDim.x + blockIdx.x; }
 
 __device__ __forceinline__ int load_id(const Teacher& t, int64_t i, int V) {
   const int64_t id = t.wide ? static_cast<const int64_t*>(t.ids)[i] : (int64_t) static_cast<const int32_t*>(t.ids)[i];
@@ -307,131 +508,170 @@ __device__ __forceinline__ int load_id(const Teacher& t, int64_t i, int V) {
 }
 
 // ------------------------------------------------------------------------------------------- teacher top-k
-// Each block selects the k best of its slice, the first block of the cluster merges the k-lists. Selection: the k-th
-// best of G >= k group maxima (a group: the vectors of kThreads / G threads) is a bound that at least k elements of
-// the slice reach and few others do (with k = 20 of 32 groups about 31 of independent values); the elements that reach it
-// are collected and ranked by counting. More than kCand of them (long runs of equal logits): k rounds of the smallest
-// key above the last, which any input ends in.
+// Each unit yields its k best keys in order; a second kernel selects the k best of a row's lists the same way. Selection:
+// the k-th largest of G >= k group maxima (a group: kThreads / G threads) is a bound that at least k values reach and few
+// others do (with k = 20 of 32 groups about 31 of independent values); what reaches it is collected and ranked by counting.
+// More than kCand (long runs of equal logits): k rounds of the smallest key above the last, which any input ends in.
+constexpr int kTopVec = 16;          // vectors per thread and unit
 constexpr int kCand = 512;
 
-// entries of a sorted list of n keys that are smaller than `key`
-__device__ __forceinline__ int below(const unsigned long long* list, int n, unsigned long long key) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (list[mid] < key) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
+struct TopScratch {
+  unsigned long long cand[kCand], warp[kWarps];
+  float gmax[kThreads];
+  float bound;
+  int count;
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) topk_kernel(const T* logits, int64_t ld, int V, int per, int k, int groups,
-                                                        float kl, int32_t* ids, float* lp) {
-  constexpr int N = Vec<T>::N;
-  extern __shared__ uint4 dyn[];
-  __shared__ unsigned long long warp_part[kWarps], part[kMaxCluster], cand[kCand];
-  __shared__ float gmax[kThreads];
-  __shared__ float s_bound;
-  __shared__ int s_count;
-  const uint32_t rank = cluster_rank(), size = cluster_size();
-  const int64_t row = blockIdx.x / size;
-  cluster_started();
-  unsigned long long* mine = reinterpret_cast<unsigned long long*>(dyn + per);   // [k], then [size * k] received
-  unsigned long long* recv = mine + k;
-  const Slice<T> s(logits + row * ld, V, per, rank);
-  load_slice(s, s.row, dyn);
-  if (threadIdx.x == 0) s_count = 0;
-  wait_slices();
-  float m = kFloor;
-  Soft soft{kFloor * kl, 0.f};
-  float best = -INFINITY;                 // as m, but below kFloor when this thread has nothing
-  for (int v = threadIdx.x; v < s.count; v += kThreads) {
-    float f[N];
-    Vec<T>::unpack(dyn[v], f);
-    best = fmaxf(best, vec_max(f));
-    add_soft(f, kl, m, soft);
-  }
-  float gm = best;
-  for (int o = kThreads / groups / 2; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-  const int lanes = kThreads / groups;
-  if (threadIdx.x % lanes == 0) gmax[threadIdx.x / lanes] = gm;
+// The k smallest keys of the block, ascending, to out[0 .. k) (kNone where there are fewer). `top`: the calling thread's
+// largest value (below kFloor: none); collect(bound, push) calls push(key) for its keys of values >= bound; after(last)
+// is its smallest key above `last`. `groups` as above. Begins and ends behind a barrier.
+template <typename Collect, typename After>
+__device__ __forceinline__ void select_keys(float top, int k, int groups, TopScratch& s, unsigned long long* out,
+                                            Collect collect, After after) {
+  const int tid = threadIdx.x, shift = __ffs(kThreads / groups) - 1;
+  float g = top;
+  for (int o = (1 << shift) >> 1; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if ((tid & ((1 << shift) - 1)) == 0) s.gmax[tid >> shift] = g;
+  if (tid == 0) s.count = 0;
   __syncthreads();
-  if (threadIdx.x < groups) {
-    const float g = gmax[threadIdx.x];
+  if (tid < groups) {
+    g = s.gmax[tid];
     int r = 0;
-    for (int j = 0; j < groups; ++j) r += gmax[j] > g || (gmax[j] == g && j < (int)threadIdx.x);
-    if (r == k - 1) s_bound = fmaxf(g, kFloor);
+    for (int j = 0; j < groups; ++j) r += s.gmax[j] > g || (s.gmax[j] == g && j < tid);
+    if (r == k - 1) s.bound = fmaxf(g, kFloor);   // kFloor: fewer than k groups hold a value, and all are collected
   }
   __syncthreads();
-  const float bound = s_bound;
-  if (best >= bound) {
-    for (int v = threadIdx.x; v < s.count; v += kThreads) {
-      float f[N];
-      Vec<T>::unpack(dyn[v], f);
-      if (vec_max(f) >= bound) {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (f[j] >= bound) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kCand) cand[at] = rank_key(f[j], s.start(v) + j);
-          }
-      }
-    }
-  }
-  for (int i = threadIdx.x; i < k; i += kThreads) mine[i] = kNone;
+  const float bound = s.bound;
+  if (top >= bound)
+    collect(bound, [&](unsigned long long key) {
+      const int at = atomicAdd(&s.count, 1);
+      if (at < kCand) s.cand[at] = key;
+    });
   __syncthreads();
-  const int n = s_count;
+  const int n = s.count;
   if (n <= kCand) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const unsigned long long key = cand[i];
+    for (int i = tid; i < n; i += kThreads) {
+      const unsigned long long key = s.cand[i];
       int r = 0;
-      for (int j = 0; j < n; ++j) r += cand[j] < key;
-      if (r < k) mine[r] = key;
+      for (int j = 0; j < n; ++j) r += s.cand[j] < key;
+      if (r < k) out[r] = key;
     }
+    for (int i = n + tid; i < k; i += kThreads) out[i] = kNone;
   } else {
-    unsigned long long last = 0;          // below every key of an unmasked logit
+    unsigned long long last = 0;     // below every key of an unmasked logit
     for (int j = 0; j < k; ++j) {
-      unsigned long long b = kNone;
-      for (int v = threadIdx.x; v < s.count; v += kThreads) {
-        float f[N];
-        Vec<T>::unpack(dyn[v], f);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const unsigned long long key = rank_key(f[i], s.start(v) + i);
-          if (f[i] >= kFloor && key > last && key < b) b = key;
-        }
-      }
-      b = warp_reduce(b, MinKey());
+      unsigned long long b = warp_reduce(after(last), MinKey());
       __syncthreads();
-      if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = b;
+      if ((tid & 31) == 0) s.warp[tid >> 5] = b;
       __syncthreads();
-      for (int w = 0; w < kWarps; ++w) b = min(b, warp_part[w]);
-      if (threadIdx.x == 0) mine[j] = b;
+      for (int w = 0; w < kWarps; ++w) b = min(b, s.warp[w]);
+      if (tid == 0) out[j] = b;
       last = b;
     }
   }
   __syncthreads();
-  cluster_peers_run();
-  for (int i = threadIdx.x; i < k; i += kThreads) st_peer(recv + rank * k + i, 0, mine[i]);
-  const Soft all = row_soft(soft, rank, size, warp_part, part);
-  if (rank != 0) return;
-  const float lse = log2f(all.sum);
-  int total = 0;
-  for (uint32_t l = 0; l < size; ++l) total += below(recv + l * k, k, kNone);
-  for (int e = threadIdx.x; e < (int)size * k; e += kThreads) {
-    const unsigned long long key = recv[e];
-    if (key == kNone) continue;
-    int r = 0;
-    for (uint32_t l = 0; l < size; ++l) r += below(recv + l * k, k, key);
-    if (r < k) {
-      ids[row * k + r] = (int32_t)(uint32_t)key;
-      lp[row * k + r] = kLn2 * (fmaf(key_value(key), kl, -all.c) - lse);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, int64_t ld, int64_t rows, int V, int k,
+                                                              int groups, float kl, unsigned long long* parts,
+                                                              unsigned long long* lists) {
+  constexpr int N = Vec<T>::N;
+  __shared__ TopScratch scratch;
+  __shared__ unsigned long long warp_part[kWarps];
+  const int tid = threadIdx.x;
+  pdl_launch_dependents();
+  const int64_t row = unit_row();
+  if (row >= rows) return;
+  const Slice<T> s(logits + row * ld, V, kTopVec * kThreads, blockIdx.x);
+  float m = kFloor, top[kTopVec / kBatch];
+  Soft soft{kFloor * kl, 0.f};
+#pragma unroll
+  for (int b = 0; b < kTopVec / kBatch; ++b) {
+    uint4 x[kBatch];
+    load_unit(s, s.row, b * kBatch * kThreads, x);
+    top[b] = unit_max<T>(x);
+    add_soft<T>(x, kl, m, soft);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
+  if ((tid & 31) == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
+  float best = top[0];
+#pragma unroll
+  for (int b = 1; b < kTopVec / kBatch; ++b) best = fmaxf(best, top[b]);
+  select_keys(
+      best, k, groups, scratch, lists + unit_index() * k,
+      [&](float bound, auto push) {                       // few threads, and few of their vectors, get here
+#pragma unroll
+        for (int b = 0; b < kTopVec / kBatch; ++b)
+          if (top[b] >= bound) {
+            uint4 x[kBatch];
+            load_unit(s, s.row, b * kBatch * kThreads, x);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+              if (packed_max<T>(x[i]) >= bound) {
+                float f[N];
+                Vec<T>::unpack(x[i], f);
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                  if (f[j] >= bound) push(rank_key(f[j], s.start(tid + (b * kBatch + i) * kThreads) + j));
+              }
+          }
+      },
+      [&](unsigned long long last) {
+        unsigned long long b = kNone;
+        for (int v = tid; v < s.count; v += kThreads)
+          for (int j = 0; j < N; ++j) {
+            const int at = s.start(v) + j;
+            if (at < 0 || at >= V) continue;
+            const float z = Vec<T>::one(s.row[at]);
+            const unsigned long long key = rank_key(z, at);
+            if (z >= kFloor && key > last && key < b) b = key;
+          }
+        return b;
+      });
+  if (tid < 32) {
+    const Soft t = join_parts(kWarps, kl, [&](int i) { return warp_part[i]; });
+    if (tid == 0) parts[unit_index()] = as_u64(t.c, t.sum);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) topk_merge_kernel(int splits, int k, int groups, float kl,
+                                                              const unsigned long long* parts,
+                                                              const unsigned long long* lists, int32_t* ids, float* lp) {
+  __shared__ TopScratch scratch;
+  __shared__ unsigned long long mine[kMaxK];
+  __shared__ float s_soft[2];
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  pdl_wait();
+  if (tid < 32) {
+    const Soft t = join_parts(splits, kl, [&](int i) { return parts[row * splits + i]; });
+    if (tid == 0) {
+      s_soft[0] = t.c;
+      s_soft[1] = log2f(t.sum);
     }
   }
-  for (int i = total + threadIdx.x; i < k; i += kThreads) {
-    ids[row * k + i] = -1;
-    lp[row * k + i] = -INFINITY;
+  const unsigned long long* keys = lists + row * splits * k;
+  const int n = splits * k;
+  unsigned long long first = kNone;
+  for (int i = tid; i < n; i += kThreads) first = min(first, keys[i]);
+  select_keys(
+      first == kNone ? -INFINITY : key_value(first), k, groups, scratch, mine,
+      [&](float bound, auto push) {
+        for (int i = tid; i < n; i += kThreads)
+          if (keys[i] != kNone && key_value(keys[i]) >= bound) push(keys[i]);
+      },
+      [&](unsigned long long last) {
+        unsigned long long b = kNone;
+        for (int i = tid; i < n; i += kThreads)
+          if (keys[i] > last && keys[i] < b) b = keys[i];
+        return b;
+      });
+  for (int i = tid; i < k; i += kThreads) {
+    const unsigned long long key = mine[i];
+    ids[row * k + i] = key == kNone ? -1 : (int32_t)(uint32_t)key;
+    lp[row * k + i] = key == kNone ? -INFINITY : kLn2 * (fmaf(key_value(key), kl, -s_soft[0]) - s_soft[1]);
   }
 }
 
@@ -448,155 +688,408 @@ __device__ __forceinline__ bool repeats(const int* ids, int i) {
   return r;
 }
 
-// One cluster per row. The teacher's tokens are replaced by -inf in shared memory once the slice is in, so the pass over
-// it sums the tail alone (a confident student's tail is lost in 1 - sum ps) and the gradient pass leaves zeros at them,
-// which the owners of the tokens then overwrite. All reads of the row lie before the cluster barrier, all writes behind
-// it: out may be the logits.
-template <typename T, bool kGrad>
-__global__ void __launch_bounds__(kThreads) kd_kernel(const T* logits, int64_t ld, int V, int per, Teacher t, float kl,
-                                                      float inv_t, const float* weight, float* loss, KdRow* stats,
-                                                      T* out, int64_t out_ld) {
-  constexpr int N = Vec<T>::N;
-  extern __shared__ uint4 dyn[];
-  __shared__ unsigned long long warp_part[kWarps], part[kMaxCluster];
-  __shared__ int s_id[kMaxK];
-  __shared__ float s_red[3][kMaxK / 32];
-  __shared__ double s_mass[kMaxK / 32];
-  const uint32_t rank = cluster_rank(), size = cluster_size();
-  const int64_t row = blockIdx.x / size;
-  cluster_started();
-  const Slice<T> s(logits + row * ld, V, per, rank);
-  load_slice(s, s.row, dyn);
-  // thread i < K holds teacher entry i
-  const int K = t.k, tid = threadIdx.x;
-  if (tid < K) s_id[tid] = load_id(t, row * K + tid, V);
-  __syncthreads();
-  int id = -1;
-  float pt = 0.f, tlp = -INFINITY, z = -INFINITY;
-  double mass = 0.0;
-  if (tid < K && s_id[tid] >= 0 && !repeats(s_id, tid)) {
-    id = s_id[tid];
-    tlp = t.lp[row * K + tid];
-    mass = exp((double)tlp);
-    pt = (float)mass;
-    z = masked(Vec<T>::one(s.row[id]));
-  }
-  wait_slices();
-  __syncthreads();
-  if (id >= 0 && s.place(id) >= 0) {
-    const uint32_t pad = Vec<T>::kPad;
-    reinterpret_cast<T*>(dyn)[s.place(id)] = *reinterpret_cast<const T*>(&pad);
-  }
-  if (tid < kMaxK) {
-    mass = warp_reduce(mass, Add());
-    if ((tid & 31) == 0) s_mass[tid >> 5] = mass;
-  }
-  __syncthreads();
-  float m = kFloor;
-  Soft soft{kFloor * kl, 0.f};
-  for (int v = tid; v < s.count; v += kThreads) {
-    float f[N];
-    Vec<T>::unpack(dyn[v], f);
-    add_soft(f, kl, m, soft);
-  }
-  cluster_peers_run();
-  const Soft tail = row_soft(soft, rank, size, warp_part, part);
-  // offset of the whole row: the teacher's tokens join here
-  if (tid < kMaxK) {
-    const float zc = warp_reduce(z, Max());
-    if ((tid & 31) == 0) s_red[0][tid >> 5] = zc;
-  }
-  __syncthreads();
-  float c = tail.c;
+constexpr int kPartVec = 16;         // vectors per thread and unit of the loss
+constexpr int kKdVec = 8;            // the same of the gradient
+constexpr int kE = kMaxK / 32;       // teacher entries per lane: entry lane + 32 i
+
+// Lists the places in a slice of the tokens id[0 .. kE) over one warp; returns their number.
+template <typename T>
+__device__ __forceinline__ int list_places(const Slice<T>& s, const int (&id)[kE], int* places) {
+  int n = 0;
 #pragma unroll
-  for (int w = 0; w < kMaxK / 32; ++w) c = fmaxf(c, s_red[0][w] * kl);
-  const float tail_sum = tail.sum * ex2(tail.c - c);
-  const float e = ex2(fmaf(z, kl, -c));
-  __syncthreads();
-  if (tid < kMaxK) {
-    const float es = warp_reduce(e, Add());
-    if ((tid & 31) == 0) s_red[0][tid >> 5] = es;
+  for (int i = 0; i < kE; ++i) {
+    const int place = id[i] < 0 ? -1 : s.place(id[i]);
+    const unsigned in = __ballot_sync(0xffffffffu, place >= 0);
+    if (place >= 0) places[n + __popc(in & ((1u << (threadIdx.x & 31)) - 1u))] = place;
+    n += __popc(in);
   }
-  __syncthreads();
-  float total = tail_sum;
-#pragma unroll
-  for (int w = 0; w < kMaxK / 32; ++w) total += s_red[0][w];
-  const bool nothing = total == 0.f;
-  const float inv_s = 1.f / total, ps = e * inv_s, ts_raw = tail_sum * inv_s;
-  const double tt_raw = 1.0 - (s_mass[0] + s_mass[1] + s_mass[2] + s_mass[3]);
-  const float tt = (float)fmax(tt_raw, (double)kTailFloor), ts = ts_raw < kTailFloor ? kTailFloor : ts_raw;
-  const float ratio = ts_raw < kTailFloor ? 0.f : tt / ts;
-  const float cc = id >= 0 ? fmaf(ratio, ps, -pt) : 0.f;
-  const float term = id >= 0 && pt != 0.f ? pt * (tlp - kLn2 * (fmaf(z, kl, -c) - log2f(total))) : 0.f;
-  if (tid < kMaxK) {
-    const float a = warp_reduce(cc, Add()), b = warp_reduce(term, Add());
-    if ((tid & 31) == 0) {
-      s_red[1][tid >> 5] = a;
-      s_red[2][tid >> 5] = b;
-    }
-  }
-  __syncthreads();
-  float csum = 0.f, l = tt * (logf(tt) - logf(ts));
-#pragma unroll
-  for (int w = 0; w < kMaxK / 32; ++w) {
-    csum += s_red[1][w];
-    l += s_red[2][w];
-  }
-  if (rank == 0 && tid == 0) {
-    loss[row] = nothing ? 0.f : l;
-    if (stats) stats[row] = nothing ? KdRow{0.f, 0.f, 0.f, 0.f} : KdRow{c, inv_s, ratio, csum};
-  }
-  if (!kGrad) return;
-  const float w = nothing ? 0.f : weight[row] * inv_t;
-  const float scale = nothing ? 0.f : -csum * inv_s * w;
-  T* o = out + row * out_ld;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(o) ^ reinterpret_cast<uintptr_t>(s.row)) & 15) == 0;
-  for (int v = tid; v < s.count; v += kThreads) {
-    float f[N];
-    Vec<T>::unpack(dyn[v], f);
-#pragma unroll
-    for (int k = 0; k < N; ++k) f[k] = scale * ex2(fmaf(f[k], kl, -c));
-    store_vec(s, o, aligned, s.start(v), f);
-  }
-  __syncthreads();
-  if (id >= 0 && s.place(id) >= 0) o[id] = Vec<T>::back(nothing ? 0.f : w * fmaf(-csum, ps, cc));
+  return n;
 }
 
-// The gradient from saved statistics: nothing to reduce, so a row is cut over independent blocks of `per` vectors.
+__device__ __forceinline__ void load_ids(const Teacher& t, int64_t row, int V, int (&id)[kE]) {
+#pragma unroll
+  for (int i = 0; i < kE; ++i) {
+    const int j = (threadIdx.x & 31) + 32 * i;
+    id[i] = j < t.k ? load_id(t, row * t.k + j, V) : -1;
+  }
+}
+
+// A row's teacher entries over the lanes of a warp.
+struct TeacherRow {
+  float lp[kE], pt[kE], z[kE];       // log-probability, probability, student logit (-inf and 0 where left out)
+  float tt;
+  unsigned kept;                     // bit i: entry lane + 32 i is in the vocabulary and not repeated
+};
 template <typename T>
-__global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64_t ld, int V, int per, int splits,
-                                                          Teacher t, float kl, float inv_t, const float* weight,
-                                                          const KdRow* stats, T* out, int64_t out_ld) {
-  constexpr int N = Vec<T>::N;
-  __shared__ int s_id[kMaxK];
-  const int64_t row = blockIdx.x / splits;
-  const Slice<T> s(logits + row * ld, V, per, blockIdx.x % splits);
-  const KdRow st = stats[row];
-  const float w = st.inv_s == 0.f ? 0.f : weight[row] * inv_t, scale = -st.csum * st.inv_s * w;
-  T* o = out + row * out_ld;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(o) ^ reinterpret_cast<uintptr_t>(s.row)) & 15) == 0;
-  const int tid = threadIdx.x;
-  if (tid < t.k) s_id[tid] = load_id(t, row * t.k + tid, V);
-#pragma unroll 4
-  for (int v = tid; v < s.count; v += kThreads) {
-    const int i0 = s.start(v);
-    float f[N];
-    if (s.full(i0)) {
-      Vec<T>::unpack(*reinterpret_cast<const uint4*>(s.row + i0), f);
-    } else {
+__device__ __forceinline__ void load_entries(const Teacher& t, int64_t row, const T* x, const int (&id)[kE],
+                                             float (&lp)[kE], float (&z)[kE]) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) f[k] = i0 + k >= 0 && i0 + k < V ? Vec<T>::one(s.row[i0 + k]) : -INFINITY;
+  for (int i = 0; i < kE; ++i) {
+    lp[i] = id[i] >= 0 ? t.lp[row * t.k + (threadIdx.x & 31) + 32 * i] : -INFINITY;
+    z[i] = id[i] >= 0 ? Vec<T>::one(x[id[i]]) : -INFINITY;
+  }
+}
+// `s_id`: kMaxK words of this warp's own.
+__device__ __forceinline__ TeacherRow teacher_row(int k, const int (&id)[kE], const float (&lp)[kE], const float (&z)[kE],
+                                                  int* s_id) {
+  TeacherRow e;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) s_id[lane + 32 * i] = id[i];
+  __syncwarp();
+  double mass = 0.0;
+  e.kept = 0;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) {
+    e.lp[i] = e.z[i] = -INFINITY;
+    e.pt[i] = 0.f;
+    if (32 * i < k) {
+      if (id[i] >= 0 && !repeats(s_id, lane + 32 * i)) {
+        e.lp[i] = lp[i];
+        e.z[i] = masked(z[i]);
+        e.kept |= 1u << i;
+      }
+      const double p = exp((double)e.lp[i]);
+      e.pt[i] = (float)p;
+      mass += p;
     }
+  }
+  e.tt = (float)fmax(1.0 - warp_reduce(mass, Add()), (double)kTailFloor);   // a difference from 1: fp64
+  __syncwarp();
+  return e;
+}
+
+// What does not depend on the tail: offset and sum of the teacher's tokens' softmax, sum pt (log pt - log-offset terms), sum
+// pt, tt.
+struct TeacherSums {
+  float c, es, l, mass, tt;
+};
+__device__ __forceinline__ TeacherSums teacher_sums(const TeacherRow& e, float kl, int k) {
+  TeacherSums r;
+  float zm = kFloor;
 #pragma unroll
-    for (int k = 0; k < N; ++k) f[k] = st.inv_s == 0.f ? 0.f : scale * ex2(fmaf(f[k], kl, -st.c));
-    store_vec(s, o, aligned, i0, f);
+  for (int i = 0; i < kE; ++i) zm = fmaxf(zm, e.z[i]);
+  r.c = warp_reduce(zm, Max()) * kl;
+  r.es = r.l = r.mass = 0.f;
+#pragma unroll
+  for (int i = 0; i < kE; ++i)
+    if (32 * i < k) {
+      const float x = fmaf(e.z[i], kl, -r.c);
+      r.es += ex2(x);
+      if (e.pt[i] != 0.f) r.l += e.pt[i] * (e.lp[i] - kLn2 * x);
+      r.mass += e.pt[i];
+    }
+  r.es = warp_reduce(r.es, Add());
+  r.l = warp_reduce(r.l, Add());
+  r.mass = warp_reduce(r.mass, Add());
+  r.tt = e.tt;
+  return r;
+}
+// Statistics and loss of a row from its tail, the softmax of all but the teacher's tokens: with ps_k = p(id_k),
+// loss = sum pt (log pt - log ps) + tt (log tt - log ts).
+__device__ __forceinline__ KdRow kd_finish(const TeacherSums& e, const Soft& tail, float& loss) {
+  const float c = fmaxf(tail.c, e.c);
+  const float tail_sum = tail.sum * ex2(tail.c - c), es = e.es * ex2(e.c - c), total = tail_sum + es;
+  if (total == 0.f) {                  // nothing in the row
+    loss = 0.f;
+    return KdRow{0.f, 0.f, 0.f, 0.f};
+  }
+  const float inv_s = 1.f / total, ts_raw = tail_sum * inv_s;
+  const float ts = ts_raw < kTailFloor ? kTailFloor : ts_raw, ratio = ts_raw < kTailFloor ? 0.f : e.tt / ts;
+  loss = e.l + e.tt * (logf(e.tt) - logf(ts));
+  if (e.mass != 0.f) loss += e.mass * kLn2 * ((c - e.c) + log2f(total));
+  return KdRow{c, inv_s, ratio, ratio * (es * inv_s) - e.mass};
+}
+// w d loss / d z at a teacher's token
+__device__ __forceinline__ float kd_pull(const KdRow& r, float w, float z, float pt, float kl) {
+  const float ps = ex2(fmaf(z, kl, -r.c)) * r.inv_s;
+  return r.inv_s == 0.f ? 0.f : w * fmaf(r.ratio - r.csum, ps, -pt);
+}
+
+// A vector with -inf in element j.
+template <typename T>
+__device__ __forceinline__ uint4 without(uint4 x, int j) {
+  constexpr int N = Vec<T>::N;
+  float f[N];
+  Vec<T>::unpack(x, f);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (k == j) f[k] = -INFINITY;
+  return Vec<T>::pack(f);
+}
+// scale 2^(z kl - c) for the elements of a vector
+template <typename T>
+__device__ __forceinline__ uint4 scaled_exp(const uint4& x, Two scale, Two minus_c, Two k2) {
+  constexpr int N = Vec<T>::N;
+  float f[N];
+  Vec<T>::unpack(x, f);
+#pragma unroll
+  for (int k = 0; k < N; k += 2) {
+    const float2 g = halves(mul2(scale, ex2_two(fma2(two(f[k], f[k + 1]), k2, minus_c))));
+    f[k] = g.x;
+    f[k + 1] = g.y;
+  }
+  return Vec<T>::pack(f);
+}
+
+// The tail's part of one unit: vectors that hold a teacher's token give it up.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) kd_parts_kernel(const T* logits, int64_t ld, int64_t rows, int V, Teacher t,
+                                                            float kl, unsigned long long* parts) {
+  constexpr int N = Vec<T>::N;
+  __shared__ int places[kMaxK], s_listed;
+  __shared__ unsigned long long warp_part[kWarps];
+  const int tid = threadIdx.x;
+  pdl_launch_dependents();
+  const int64_t row = unit_row();
+  if (row >= rows) return;
+  const Slice<T> s(logits + row * ld, V, kPartVec * kThreads, blockIdx.x);
+  uint4 x[kBatch];
+  load_unit(s, x);
+  if (tid < 32) {
+    int id[kE];
+    load_ids(t, row, V, id);
+    const int n = list_places(s, id, places);
+    if (tid == 0) s_listed = n;
   }
   __syncthreads();
-  if (tid < t.k && s_id[tid] >= 0 && s.place(s_id[tid]) >= 0 && !repeats(s_id, tid)) {
-    const int id = s_id[tid];
-    const float ps = ex2(fmaf(masked(Vec<T>::one(s.row[id])), kl, -st.c)) * st.inv_s;
+  const int listed = s_listed;
+  float m = kFloor;
+  Soft soft{kFloor * kl, 0.f};
+#pragma unroll
+  for (int b = 0; b < kPartVec / kBatch; ++b) {
+    if (b) load_unit(s, s.row, b * kBatch * kThreads, x);
+    for (int j = 0; j < listed; ++j) {
+      const int v = places[j] / N - b * kBatch * kThreads;
+      if (v % kThreads == tid)
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          if (v == tid + i * kThreads) x[i] = without<T>(x[i], places[j] % N);
+    }
+    add_soft<T>(x, kl, m, soft);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
+  if ((tid & 31) == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
+  __syncthreads();
+  if (tid < 32) {
+    const Soft r = join_parts(kWarps, kl, [&](int i) { return warp_part[i]; });
+    if (tid == 0) parts[unit_index()] = as_u64(r.c, r.sum);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32) kd_loss_kernel(const T* logits, int64_t ld, int splits, int V, Teacher t, float kl,
+                                                     const unsigned long long* parts, float* loss, KdRow* stats) {
+  __shared__ int s_id[kMaxK];
+  const int64_t row = blockIdx.x;
+  int id[kE];
+  load_ids(t, row, V, id);
+  float lp[kE], z[kE];
+  load_entries(t, row, logits + row * ld, id, lp, z);
+  const TeacherSums sums = teacher_sums(teacher_row(t.k, id, lp, z, s_id), kl, t.k);
+  pdl_wait();
+  const Soft tail = join_parts(splits, kl, [&](int i) { return parts[row * splits + i]; });
+  float l;
+  const KdRow r = kd_finish(sums, tail, l);
+  if (threadIdx.x == 0) {
+    loss[row] = l;
+    if (stats) stats[row] = r;
+  }
+}
+
+// What kd_grad_kernel needs of the rows' teachers, prepared by a small kernel before it: with the student's logits at the
+// teacher's tokens read there, the gradient may go over the logits.
+struct KdRows {
+  int* id;                           // [rows, k], -1: left out
+  float *z, *pt;                     // [rows, k]
+  float* sums;                       // [rows, 6] TeacherSums, weight / T
+};
+template <typename T>
+__global__ void __launch_bounds__(32) kd_prepare_kernel(const T* logits, int64_t ld, int V, Teacher t, float kl, float inv_t,
+                                                        const float* weight, KdRows r) {
+  __shared__ int s_id[kMaxK];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  pdl_launch_dependents();
+  int id[kE];
+  float lp[kE], z[kE];
+  load_ids(t, row, V, id);
+  load_entries(t, row, logits + row * ld, id, lp, z);
+  const TeacherRow e = teacher_row(t.k, id, lp, z, s_id);
+#pragma unroll
+  for (int i = 0; i < kE; ++i)
+    if (lane + 32 * i < t.k) {
+      const int64_t at = row * t.k + lane + 32 * i;
+      r.id[at] = e.kept >> i & 1 ? id[i] : -1;
+      r.z[at] = e.z[i];
+      r.pt[at] = e.pt[i];
+    }
+  const TeacherSums s = teacher_sums(e, kl, t.k);
+  if (lane == 0) {
+    float* o = r.sums + 6 * row;
+    o[0] = s.c;
+    o[1] = s.es;
+    o[2] = s.l;
+    o[3] = s.mass;
+    o[4] = s.tt;
+    o[5] = weight[row] * inv_t;
+  }
+}
+
+// The teacher's tokens in a block's share of a row.
+struct ShareIds {
+  int n, id[kMaxK];
+  float z[kMaxK], pt[kMaxK];
+};
+
+// Loss and gradient of a row by one block or cluster. The owner of a teacher's token takes it out (-inf) before the first
+// look, which so sums the tail alone (a confident student's tail is lost in 1 - sum ps); after the second look it writes
+// the token's gradient.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads, kRowBlocks) kd_grad_kernel(const T* logits, int64_t ld, int V, int keep,
+                                                                          int k, float kl, float* loss, T* out,
+                                                                          int64_t out_ld, KdRows r) {
+  constexpr int N = Vec<T>::N;
+  extern __shared__ uint4 dyn[];
+  __shared__ unsigned long long warp_part[kRowWarps], part[kMaxCluster];
+  __shared__ ShareIds list;
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  const int64_t row = blockIdx.x / size;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const Share<T> s(logits + row * ld, V, rank, size, keep);
+  cluster_started();
+  copy_kept(s, s.row, dyn);
+  pdl_wait();
+  if (tid < 32) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      const int64_t at = row * k + lane + 32 * i;
+      const int id = lane + 32 * i < k ? r.id[at] : -1;
+      const bool in = id >= 0 && s.holds(id);
+      const unsigned all = __ballot_sync(0xffffffffu, in);
+      if (in) {
+        const int j = n + __popc(all & ((1u << lane) - 1u));
+        list.id[j] = id;
+        list.z[j] = r.z[at];
+        list.pt[j] = r.pt[at];
+      }
+      n += __popc(all);
+    }
+    if (lane == 0) list.n = n;
+  }
+  __syncthreads();
+  const int listed = list.n;
+  int own = 0, own_v = 0;              // this thread's teacher tokens among the streamed vectors, the vector of one
+  for (int j = 0; j < listed; ++j)
+    if (s.owns(list.id[j]) && (list.id[j] - s.e0) / N >= s.kept) {
+      ++own;
+      own_v = (list.id[j] - s.e0) / N;
+    }
+  float m = kFloor;
+  Soft soft{kFloor * kl, 0.f};
+  for (int v = s.kept + tid; v < s.n; v += kRound) {
+    uint4 x[4];
+    stream(s, s.row, true, v, x);
+    if (own > 1 || (own == 1 && own_v >= v && own_v < v + kRound))
+      for (int j = 0; j < listed; ++j) {
+        const int at = list.id[j] - s.e0;
+        if (s.owns(list.id[j]))
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (at / N == v + i * kRowThreads) x[i] = without<T>(x[i], at % N);
+      }
+    add_soft<T>(x, kl, m, soft);
+  }
+  const int single = s.single();
+  bool single_in = single >= 0;
+  if (single_in) {
+    for (int j = 0; j < listed; ++j) single_in &= list.id[j] != single;
+    if (single_in) {
+      uint4 x[1] = {make_uint4(Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad)};
+      *reinterpret_cast<T*>(x) = s.row[single];
+      add_soft<T>(x, kl, m, soft);
+    }
+  }
+  wait_copies();
+  for (int j = 0; j < listed; ++j) {
+    const int at = list.id[j] - s.e0;
+    if (s.owns(list.id[j]) && at / N < s.kept) dyn[at / N] = without<T>(dyn[at / N], at % N);
+  }
+  for (int v = tid; v < s.kept; v += kRound) {
+    const uint4 x[4] = {dyn[v], dyn[v + kRowThreads], dyn[v + 2 * kRowThreads], dyn[v + 3 * kRowThreads]};
+    add_soft<T>(x, kl, m, soft);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
+  if (lane == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
+  __syncthreads();
+  cluster_peers_run();
+  if (tid < 32) {
+    const Soft b = join_parts(kRowWarps, kl, [&](int i) { return warp_part[i]; });
+    if (lane < (int)size) st_peer(part + rank, lane, as_u64(b.c, b.sum));
+  }
+  cluster_sync();
+  const Soft tail = join_parts(size, kl, [&](int i) { return part[i]; });
+  const float* sums = r.sums + 6 * row;
+  const float w = sums[5];
+  float l;
+  const KdRow f = kd_finish(TeacherSums{sums[0], sums[1], sums[2], sums[3], sums[4]}, tail, l);
+  if (rank == 0 && tid == 0) loss[row] = l;
+  T* o = out + row * out_ld;
+  const Two scale = two(f.inv_s == 0.f ? 0.f : -f.csum * f.inv_s * w), c2 = two(-f.c), k2 = two(kl);
+  if (same_phase<T>(o, s.row)) {
+    uint4* p = reinterpret_cast<uint4*>(o + s.e0);
+    for (int v = s.kept + tid; v < s.n; v += kRound) {
+      uint4 x[4];
+      stream(s, s.row, true, v, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v + i * kRowThreads < s.n) __stcs(p + v + i * kRowThreads, scaled_exp<T>(x[i], scale, c2, k2));
+    }
+    for (int v = tid; v < s.kept; v += kRound)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) __stcs(p + v + i * kRowThreads, scaled_exp<T>(dyn[v + i * kRowThreads], scale, c2, k2));
+  } else {
+    for (int v = tid; v < s.n; v += kRowThreads) {
+      const uint4 u = scaled_exp<T>(v < s.kept ? dyn[v] : __ldcg(reinterpret_cast<const uint4*>(s.row + s.e0) + v), scale, c2, k2);
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[s.e0 + v * N + j] = reinterpret_cast<const T*>(&u)[j];
+    }
+  }
+  if (single_in) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<T*>(&x) = s.row[single];
+    x = scaled_exp<T>(x, scale, c2, k2);
+    o[single] = *reinterpret_cast<const T*>(&x);
+  }
+  for (int j = 0; j < listed; ++j)
+    if (s.owns(list.id[j]) || list.id[j] == single) o[list.id[j]] = Vec<T>::back(kd_pull(f, w, list.z[j], list.pt[j], kl));
+}
+
+// The gradient from saved statistics.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64_t ld, int64_t rows, int V, Teacher t,
+                                                          float kl, float inv_t, const float* weight,
+                                                          const KdRow* stats, T* out, int64_t out_ld) {
+  const int64_t row = unit_row();
+  if (row >= rows) return;
+  const Slice<T> s(logits + row * ld, V, kKdVec * kThreads, blockIdx.x);
+  uint4 x[kKdVec];
+  load_unit(s, x);
+  const KdRow st = stats[row];
+  const float w = st.inv_s == 0.f ? 0.f : weight[row] * inv_t;
+  T* o = out + row * out_ld;
+  const int tid = threadIdx.x, id = tid < t.k ? load_id(t, row * t.k + tid, V) : -1;
+  const Two scale = two(st.inv_s == 0.f ? 0.f : -st.csum * st.inv_s * w), c2 = two(-st.c), k2 = two(kl);
+  store_unit<kKdVec>(s, o, [&](int i) { return scaled_exp<T>(x[i], scale, c2, k2); });
+  __syncthreads();
+  if (id >= 0 && s.place(id) >= 0) {
+    bool repeated = false;
+    for (int j = 0; j < tid; ++j) repeated |= load_id(t, row * t.k + j, V) == id;
     const float pt = (float)exp((double)t.lp[row * t.k + tid]);
-    o[id] = Vec<T>::back(st.inv_s == 0.f ? 0.f : w * fmaf(st.ratio - st.csum, ps, -pt));
+    if (!repeated) o[id] = Vec<T>::back(kd_pull(st, w, masked(Vec<T>::one(s.row[id])), pt, kl));
   }
 }
 
@@ -630,158 +1123,206 @@ __device__ __forceinline__ Pair shfl_xor(const Pair& a, int o) {
   return {shfl_xor(a.q, o), shfl_xor(a.p, o), __shfl_xor_sync(0xffffffffu, a.d, o)};
 }
 
+constexpr int kPairVec = 4;          // vectors per thread, unit and side of the gradient
+
+template <typename Load>
+__device__ __forceinline__ Pair join_pairs(int n, float kl, Load load) {
+  Pair t{{kFloor * kl, 0.f}, {kFloor * kl, 0.f}, 0.f};
+  for (int i = threadIdx.x & 31; i < n; i += 32) t = join(t, load(i));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) t = join(t, shfl_xor(t, o));
+  return t;
+}
+// Adds pairs of vectors to a thread's running Pair with maxima mq, mp.
+template <typename T, int kVec>
+__device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&xp)[kVec], float kl, float& mq, float& mp,
+                                         Pair& a) {
+  constexpr int N = Vec<T>::N;
+  const float vq = unit_max<T>(xq), vp = unit_max<T>(xp);
+  float low = packed_min<T>(xq[0]);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) low = fminf(low, fminf(packed_min<T>(xq[i]), packed_min<T>(xp[i])));
+  if (vq > mq || vp > mp) {
+    mq = fmaxf(mq, vq);
+    mp = fmaxf(mp, vp);
+    a = join(a, Pair{{mq * kl, 0.f}, {mp * kl, 0.f}, 0.f});
+  }
+  const Two k2 = two(kl), cq = two(-a.q.c), cp = two(-a.p.c), minus = two(-1.f);
+  Two sq = two(0.f), sp = two(0.f), d = two(0.f);
+  const auto look = [&](auto guarded) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      float q[N], p[N];
+      Vec<T>::unpack(xq[i], q);
+      Vec<T>::unpack(xp[i], p);
+#pragma unroll
+      for (int k = 0; k < N; k += 2) {
+        if (guarded) {
+          q[k] = masked(q[k]);
+          q[k + 1] = masked(q[k + 1]);
+        }
+        const Two eq = fma2(two(q[k], q[k + 1]), k2, cq), ep = fma2(two(p[k], p[k + 1]), k2, cp), w = ex2_two(ep);
+        sq = add2(sq, ex2_two(eq));
+        sp = add2(sp, w);
+        const Two gap = fma2(eq, minus, ep);
+        if (guarded) {
+          const float2 wf = halves(w), gf = halves(gap);
+          d = add2(d, two(wf.x > 0.f ? wf.x * gf.x : 0.f, wf.y > 0.f ? wf.y * gf.y : 0.f));
+        } else {
+          d = fma2(w, gap, d);
+        }
+      }
+    }
+  };
+  // masked logits: 0 times an infinite gap is 0, and a token that only the draft masks makes KL infinite, whatever masks it
+  if (low >= kFloor) look(std::false_type());
+  else look(std::true_type());
+  a.q.sum += sum(sq);
+  a.p.sum += sum(sp);
+  a.d += sum(d);
+}
+
+// One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) accept_kernel(const T* draft, int64_t ldq, const T* target, int64_t ldp,
-                                                          int V, int per, float kl, float* alpha, float* out_kl,
-                                                          AcceptRow* stats) {
+__global__ void __launch_bounds__(kRowThreads, kRowBlocks) accept_kernel(const T* draft, int64_t ldq, const T* target,
+                                                                         int64_t ldp, int V, int keep, float kl,
+                                                                         float* alpha, float* out_kl, AcceptRow* stats) {
   constexpr int N = Vec<T>::N;
   extern __shared__ uint4 dyn[];
-  __shared__ unsigned long long part[kMaxCluster][3], sums[kMaxCluster];
-  __shared__ Pair warp_pair[kWarps];
-  __shared__ float2 warp_sum[kWarps];
+  __shared__ unsigned long long part[3][kMaxCluster], sums[kMaxCluster];
+  __shared__ Pair warp_pair[kRowWarps];
+  __shared__ float2 warp_sum[kRowWarps];
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int64_t row = blockIdx.x / size;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const T* other = target + row * ldp;
+  const Share<T> s(draft + row * ldq, V, rank, size, keep);
+  const bool same = same_phase(other, s.row);
+  const uint4 *dq = dyn, *dp = dyn + s.kept;
   cluster_started();
-  uint4* dp = dyn + per;
-  const Slice<T> s(draft + row * ldq, V, per, rank);
-  load_slice(s, s.row, dyn);
-  load_slice(s, target + row * ldp, dp);
-  wait_slices();
-  const int tid = threadIdx.x;
+  copy_kept(s, s.row, dyn);
+  copy_kept(s, other, dyn + s.kept);
+  const int single = s.single();
+  uint4 lone[2][1];
+  if (single >= 0) {
+    lone[0][0] = lone[1][0] = make_uint4(Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad);
+    *reinterpret_cast<T*>(lone[0]) = s.row[single];
+    *reinterpret_cast<T*>(lone[1]) = other[single];
+  }
   float mq = kFloor, mp = kFloor;
   Pair a{{kFloor * kl, 0.f}, {kFloor * kl, 0.f}, 0.f};
-  for (int v = tid; v < s.count; v += kThreads) {
-    float q[N], p[N];
-    Vec<T>::unpack(dyn[v], q);
-    Vec<T>::unpack(dp[v], p);
-    const float vq = vec_max(q), vp = vec_max(p);
-    if (vq > mq || vp > mp) {
-      mq = fmaxf(mq, vq);
-      mp = fmaxf(mp, vp);
-      a = join(a, Pair{{mq * kl, 0.f}, {mp * kl, 0.f}, 0.f});
-    }
-    if (vec_min(q) < kFloor) {            // a token that only the draft masks makes KL infinite, whatever masks it
-#pragma unroll
-      for (int k = 0; k < N; ++k) q[k] = masked(q[k]);
-    }
-    float sq = 0.f, sp = 0.f, d = 0.f;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float xq = fmaf(q[k], kl, -a.q.c), xp = fmaf(p[k], kl, -a.p.c), ep = ex2(xp);
-      sq += ex2(xq);
-      sp += ep;
-      d += ep > 0.f ? ep * (xp - xq) : 0.f;
-    }
-    a.q.sum += sq;
-    a.p.sum += sp;
-    a.d += d;
+  for (int v = s.kept + tid; v < s.n; v += 2 * kRowThreads) {
+    uint4 xq[2], xp[2];
+    stream(s, s.row, true, v, xq);
+    stream(s, other, same, v, xp);
+    add_pair<T>(xq, xp, kl, mq, mp, a);
+  }
+  if (single >= 0) add_pair<T>(lone[0], lone[1], kl, mq, mp, a);
+  wait_copies();
+  for (int v = tid; v < s.kept; v += 2 * kRowThreads) {
+    const uint4 xq[2] = {dq[v], dq[v + kRowThreads]}, xp[2] = {dp[v], dp[v + kRowThreads]};
+    add_pair<T>(xq, xp, kl, mq, mp, a);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) a = join(a, shfl_xor(a, o));
-  if ((tid & 31) == 0) warp_pair[tid >> 5] = a;
+  if (lane == 0) warp_pair[tid >> 5] = a;
   __syncthreads();
   cluster_peers_run();
   if (tid < 32) {
-    a = warp_pair[tid & (kWarps - 1)];
-#pragma unroll
-    for (int o = kWarps / 2; o; o >>= 1) a = join(a, shfl_xor(a, o));
-    if (tid < (int)size) {
-      st_peer(&part[rank][0], tid, as_u64(a.q.c, a.q.sum));
-      st_peer(&part[rank][1], tid, as_u64(a.p.c, a.p.sum));
-      st_peer(&part[rank][2], tid, as_u64(a.d, 0.f));
+    a = join_pairs(kRowWarps, kl, [&](int i) { return warp_pair[i]; });
+    if (lane < (int)size) {
+      st_peer(&part[0][rank], lane, as_u64(a.q.c, a.q.sum));
+      st_peer(&part[1][rank], lane, as_u64(a.p.c, a.p.sum));
+      st_peer(&part[2][rank], lane, as_u64(a.d, 0.f));
     }
   }
   cluster_sync();
-  for (uint32_t i = 0; i < size; ++i) {
-    const unsigned long long u = part[i][0], w = part[i][1];
-    const Pair b{{__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32))},
-                 {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))},
-                 __uint_as_float((uint32_t)part[i][2])};
-    a = i ? join(a, b) : b;
-  }
-  const double lq = log2((double)a.q.sum), lp = log2((double)a.p.sum);
-  const double bq = a.q.c + lq, bp = a.p.c + lp;
-  const float rq = (float)bq, rp = (float)bp;
-  float below_p = 0.f, above = 0.f;        // sums of min(q, p) where q <= p and where q > p
-  for (int v = tid; v < s.count; v += kThreads) {
+  a = join_pairs(size, kl, [&](int i) { return Pair{as_soft(part[0][i]), as_soft(part[1][i]), as_soft(part[2][i]).c}; });
+  const float rq = a.q.c + log2f(a.q.sum), rp = a.p.c + log2f(a.p.sum);
+  float under = 0.f, over = 0.f;             // sums of min(q, p) where q <= p and where q > p
+  const Two k2 = two(kl), bq = two(-rq), bp = two(-rp);
+  const auto look = [&](const uint4& uq, const uint4& up) {
     float q[N], p[N];
-    Vec<T>::unpack(dyn[v], q);
-    Vec<T>::unpack(dp[v], p);
-    float x = 0.f, y = 0.f;
+    Vec<T>::unpack(uq, q);
+    Vec<T>::unpack(up, p);
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float xq = fmaf(q[k], kl, -rq), xp = fmaf(p[k], kl, -rp), e = ex2(fminf(xq, xp));
-      x += xq <= xp ? e : 0.f;
-      y += xq <= xp ? 0.f : e;
+    for (int k = 0; k < N; k += 2) {
+      const float2 eq = halves(fma2(two(q[k], q[k + 1]), k2, bq)), ep = halves(fma2(two(p[k], p[k + 1]), k2, bp));
+      const float e0 = ex2(fminf(eq.x, ep.x)), e1 = ex2(fminf(eq.y, ep.y));
+      if (eq.x <= ep.x) under += e0;
+      else over += e0;
+      if (eq.y <= ep.y) under += e1;
+      else over += e1;
     }
-    below_p += x;
-    above += y;
+  };
+  for (int v = s.kept + tid; v < s.n; v += 2 * kRowThreads) {
+    uint4 xq[2], xp[2];
+    stream(s, s.row, true, v, xq);
+    stream(s, other, same, v, xp);
+    look(xq[0], xp[0]);
+    look(xq[1], xp[1]);                      // padding adds 0
   }
-  below_p = warp_reduce(below_p, Add());
-  above = warp_reduce(above, Add());
-  if ((tid & 31) == 0) warp_sum[tid >> 5] = make_float2(below_p, above);
+  if (single >= 0) look(lone[0][0], lone[1][0]);
+#pragma unroll 2
+  for (int v = tid; v < s.kept; v += kRowThreads) look(dq[v], dp[v]);
+  under = warp_reduce(under, Add());
+  over = warp_reduce(over, Add());
+  if (lane == 0) warp_sum[tid >> 5] = make_float2(under, over);
   __syncthreads();
-  if (tid == 0) {
-    float2 t = warp_sum[0];
-    for (int w = 1; w < kWarps; ++w) {
-      t.x += warp_sum[w].x;
-      t.y += warp_sum[w].y;
-    }
-    st_peer(sums + rank, 0, as_u64(t.x, t.y));
+  if (tid < 32) {
+    float2 w = lane < kRowWarps ? warp_sum[lane] : make_float2(0.f, 0.f);
+    w.x = warp_reduce(w.x, Add());
+    w.y = warp_reduce(w.y, Add());
+    if (lane == 0) st_peer(sums + rank, 0, as_u64(w.x, w.y));
   }
   cluster_sync();
   if (rank != 0 || tid != 0) return;
   float x = 0.f, y = 0.f;
   for (uint32_t i = 0; i < size; ++i) {
-    x += __uint_as_float((uint32_t)sums[i]);
-    y += __uint_as_float((uint32_t)(sums[i] >> 32));
+    x += as_soft(sums[i]).c;
+    y += as_soft(sums[i]).sum;
   }
+  const double lq = log2((double)a.q.sum), lp = log2((double)a.p.sum);
+  const float fq = exp2f((float)((double)rq - (a.q.c + lq))), fp = exp2f((float)((double)rp - (a.p.c + lp)));
   const bool nothing = a.q.sum == 0.f || a.p.sum == 0.f;
-  const float fq = exp2f((float)((double)rq - bq)), fp = exp2f((float)((double)rp - bp));
   const bool nan = isnan(a.q.sum) || isnan(a.p.sum);      // the minimum drops a NaN operand
   alpha[row] = nothing ? 0.f : nan ? NAN : fq * x + fp * y;
-  out_kl[row] = nothing ? 0.f : (float)((double)kLn2 * ((double)a.d / a.p.sum + (lq - lp)));
+  out_kl[row] = nothing ? 0.f : (float)((double)kLn2 * ((double)a.d / a.p.sum + lq - lp));
   if (stats) stats[row] = nothing ? AcceptRow{0.f, 0.f, 0.f, 0.f, 0.f} : AcceptRow{rq, fq, rp, fp, fq * x};
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, int64_t ldq, const T* target, int64_t ldp,
-                                                              int V, int per, int splits, float kl, float inv_t,
+                                                              int64_t rows, int V, float kl, float inv_t,
                                                               const AcceptRow* stats, const float* g_alpha,
                                                               const float* g_kl, T* out, int64_t out_ld) {
   constexpr int N = Vec<T>::N;
-  const int64_t row = blockIdx.x / splits;
-  const Slice<T> s(draft + row * ldq, V, per, blockIdx.x % splits);
-  const T* xp_row = target + row * ldp;
+  const int64_t row = unit_row();
+  if (row >= rows) return;
+  const Slice<T> s(draft + row * ldq, V, kPairVec * kThreads, blockIdx.x);
+  uint4 xq[kPairVec], xp[kPairVec];
+  load_unit(s, xq);
+  load_unit(s, target + row * ldp, 0, xp);
   const AcceptRow st = stats[row];
   const bool nothing = st.fq == 0.f;
   const float ga = g_alpha[row] * inv_t, gk = g_kl[row] * inv_t;
-  const float under = st.fq * (ga * (1.f - st.a) + gk), over = st.fq * (gk - ga * st.a), kp = gk * st.fp;
-  T* o = out + row * out_ld;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(o) ^ reinterpret_cast<uintptr_t>(s.row)) & 15) == 0;
-  const bool same = ((reinterpret_cast<uintptr_t>(xp_row) ^ reinterpret_cast<uintptr_t>(s.row)) & 15) == 0;
-#pragma unroll 2
-  for (int v = threadIdx.x; v < s.count; v += kThreads) {
-    const int i0 = s.start(v);
+  const float under = st.fq * (ga * (1.f - st.a) + gk), over = st.fq * (gk - ga * st.a);
+  const Two k2 = two(kl), bq = two(-st.bq), bp = two(-st.bp), kp = two(-gk * st.fp);
+  store_unit<kPairVec>(s, out + row * out_ld, [&](int i) {
     float q[N], p[N];
-    if (same && s.full(i0)) {
-      Vec<T>::unpack(*reinterpret_cast<const uint4*>(s.row + i0), q);
-      Vec<T>::unpack(*reinterpret_cast<const uint4*>(xp_row + i0), p);
-    } else {
+    Vec<T>::unpack(xq[i], q);
+    Vec<T>::unpack(xp[i], p);
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const bool in = i0 + k >= 0 && i0 + k < V;
-        q[k] = in ? Vec<T>::one(s.row[i0 + k]) : -INFINITY;
-        p[k] = in ? Vec<T>::one(xp_row[i0 + k]) : -INFINITY;
-      }
+    for (int k = 0; k < N; k += 2) {
+      const Two eq = fma2(two(q[k], q[k + 1]), k2, bq), ep = fma2(two(p[k], p[k + 1]), k2, bp);
+      const float2 fq = halves(eq), fp = halves(ep);
+      const float2 g = halves(fma2(ex2_two(eq), two(fq.x <= fp.x ? under : over, fq.y <= fp.y ? under : over),
+                                   mul2(kp, ex2_two(ep))));
+      q[k] = nothing ? 0.f : g.x;
+      q[k + 1] = nothing ? 0.f : g.y;
     }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float xq = fmaf(q[k], kl, -st.bq), xp = fmaf(p[k], kl, -st.bp);
-      q[k] = nothing ? 0.f : ex2(xq) * (xq <= xp ? under : over) - kp * ex2(xp);
-    }
-    store_vec(s, o, aligned, i0, q);
-  }
+    return Vec<T>::pack(q);
+  });
 }
 
 // ------------------------------------------------------------------------------------------- draft verification
@@ -822,35 +1363,21 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
   const T* row = draft ? static_cast<const T*>(a.draft_logits) + b * a.draft_b + (j - a.k - 1) * a.draft_j
                        : static_cast<const T*>(a.logits) + b * a.logits_b + j * a.logits_j;
   const Slice<T> s(row, a.V, kUnroll * kThreads, split);
-  uint4 u[kUnroll];
-#pragma unroll
-  for (int i = 0; i < kUnroll; ++i) {
-    const int v = threadIdx.x + i * kThreads, i0 = s.start(v);
-    u[i] = make_uint4(Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad);
-    if (v < s.count) {
-      if (s.full(i0)) {
-        u[i] = *reinterpret_cast<const uint4*>(row + i0);
-      } else {
-        float f[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) f[k] = i0 + k >= 0 && i0 + k < a.V ? Vec<T>::one(row[i0 + k]) : -INFINITY;
-        u[i] = Vec<T>::pack(f);
-      }
-    }
-  }
+  uint4 x[kUnroll];
+  load_unit(s, x);
+  const float top = unit_max<T>(x);
   unsigned long long res;
   if (greedy) {
     res = kNone;
-    float m = -INFINITY;
+    const float best = warp_reduce(top, Max());
+    if (top == best && best >= kFloor) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      float f[N];
-      Vec<T>::unpack(u[i], f);
-      if (vec_max(f) > m) {
-        m = vec_max(f);
+      for (int i = kUnroll - 1; i >= 0; --i) {          // ends at the thread's first element of that value
+        float f[N];
+        Vec<T>::unpack(x[i], f);
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-          if (f[k] >= kFloor) res = min(res, rank_key(f[k], s.start(threadIdx.x + i * kThreads) + k));
+        for (int k = N - 1; k >= 0; --k)
+          if (f[k] == best) res = rank_key(best, s.start(threadIdx.x + i * kThreads) + k);
       }
     }
     res = warp_reduce(res, MinKey());
@@ -859,23 +1386,12 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
     for (int w = 0; w < kWarps; ++w) res = min(res, warp_part[w]);
   } else {
     const float kl = kLog2e / temp;
-    float m = kFloor;
-    Soft soft{kFloor * kl, 0.f};
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      float f[N];
-      Vec<T>::unpack(u[i], f);
-      add_soft(f, kl, m, soft);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
+    const Soft soft = warp_soft<T>(x, fmaxf(top, kFloor), kl);
     if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = as_u64(soft.c, soft.sum);
     __syncthreads();
-    const unsigned long long w = warp_part[threadIdx.x & (kWarps - 1)];
-    soft = {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))};
-#pragma unroll
-    for (int o = kWarps / 2; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
-    res = as_u64(soft.c, soft.sum);
+    if (threadIdx.x >= 32) return;
+    const Soft t = join_parts(kWarps, kl, [&](int i) { return warp_part[i]; });
+    res = as_u64(t.c, t.sum);
   }
   if (threadIdx.x == 0) static_cast<unsigned long long*>(a.workspace)[blockIdx.x] = res;
 }
@@ -1025,41 +1541,66 @@ int sm_count() {
   return n;
 }
 
-// Blocks per row and vectors per block. `bytes`: of one vector position over all tensors that a block keeps.
-struct Plan {
-  int cluster, per;
-};
-Plan plan_of(int64_t rows, int V, int lanes, int bytes) {
-  const int total = (V + lanes - 1) / lanes + 1;     // + 1: a row that starts off a boundary
-  int c = 1;
-  while (c < 8 && (int64_t)total * bytes > (int64_t)c * 40960) c *= 2;
-  while (c < kMaxCluster && (int64_t)total * bytes > (int64_t)c * 204800) c *= 2;
-  while (c < kMaxCluster && rows * c < sm_count() && total > 2 * kThreads * c) c *= 2;
-  return {c, (total + c - 1) / c};
+// Units per row of `z`: a row that starts off a 16-byte boundary may touch one vector more.
+int splits_of(Type type, Logits z, int64_t rows, int V, int unit) {
+  const int lanes = type == F32 ? 4 : 8;
+  const bool aligned = (reinterpret_cast<uintptr_t>(z.p) & 15) == 0 && (rows == 1 || z.ld % lanes == 0);
+  return ((V + lanes - 1) / lanes + (aligned ? 0 : 1) + unit - 1) / unit;
 }
 
+// Blocks per row (a cluster) and vectors that a block keeps, in the kernels that look twice; `sides` tensors share a block.
+struct Plan {
+  int cluster, keep, smem;
+};
+Plan plan_of(Type type, int64_t rows, int V, int sides) {
+  const int total = V / (type == F32 ? 4 : 8) + 1;
+  const int64_t slots = kRowBlocks * sm_count();
+  // enough blocks per row that what all running blocks do not keep stays in half of L2, then as few as leave no more than
+  // a seventh of the slots idle over all waves
+  int c = 1;
+  while (c < kMaxCluster && (total * sides / c - kKeep) * 16ll * slots > 64 << 20) c *= 2;
+  while (c < kMaxCluster && total * sides > kRowThreads * c && rows * c * 7 < (rows * c + slots - 1) / slots * slots * 6) c *= 2;
+  const int per = (total + c - 1) / c, keep = std::min(per, kKeep / sides) / kRound * kRound;
+  return {c, keep, keep * sides * 16};
+}
+
+cudaError_t allow(const void* f, int cluster, size_t smem) {
+  cudaError_t e = cudaSuccess;
+  if (smem > 32768) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e;
+}
+
+struct Shape {
+  int64_t blocks;
+  int units = 0;               // per row: `blocks` rows of them
+  int threads = kThreads, cluster = 1;
+  size_t smem = 0;
+  bool early = false;          // may start while the kernel before it runs (griddepcontrol.wait orders them)
+};
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), int64_t blocks, int threads, int cluster, size_t smem, bool early,
-                   cudaStream_t stream, A... args) {
-  const void* f = reinterpret_cast<const void*>(kernel);
-  cudaError_t e;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if (smem > 32768 && (e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
-    return e;
-  if (cluster > 8 && (e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
-    return e;
+cudaError_t launch(void (*kernel)(P...), const Shape& s, cudaStream_t stream, A... args) {
+  cudaError_t e = allow(reinterpret_cast<const void*>(kernel), s.cluster, s.smem);
+  if (e != cudaSuccess) return e;
+  if (s.blocks < 1 || s.blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3((unsigned)s.blocks);
+  if (s.units) {
+    const unsigned y = (unsigned)std::min<int64_t>(s.blocks, 32768);
+    cfg.gridDim = dim3(s.units, y, (unsigned)((s.blocks + y - 1) / y));
+  }
+  cfg.blockDim = dim3(s.threads);
+  cfg.dynamicSmemBytes = s.smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[3];
   int n = 0;
-  attr[n].id = cudaLaunchAttributeClusterDimension;
-  attr[n].val.clusterDim.x = cluster;
-  attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-  ++n;
-  if (early) {
+  if (s.cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = s.cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (s.early) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;
@@ -1076,61 +1617,145 @@ cudaError_t by_type(Type type, F&& f) {
   return f(__nv_bfloat16());
 }
 
-constexpr int kBwdVectors = 8;       // vectors per thread of an elementwise gradient block
+// Hands out the workspace piece by piece, 16-byte aligned.
+struct Carver {
+  char* p;
+  size_t used = 0;
+  template <typename T> T* take(size_t n) {
+    T* r = reinterpret_cast<T*>(p + used);
+    used += (n * sizeof(T) + 15) & ~size_t(15);
+    return r;
+  }
+};
+struct TopWork {
+  unsigned long long *parts, *lists;
+  size_t bytes;
+};
+TopWork carve_topk(int64_t units, int k, void* p) {
+  Carver c{static_cast<char*>(p)};
+  TopWork t{};
+  t.parts = c.take<unsigned long long>(units);
+  t.lists = c.take<unsigned long long>(units * k);
+  t.bytes = c.used;
+  return t;
+}
+KdRows carve_kd(int64_t rows, int k, void* p, size_t& bytes) {
+  Carver c{static_cast<char*>(p)};
+  KdRows r{};
+  r.id = c.take<int>(rows * k);
+  r.z = c.take<float>(rows * k);
+  r.pt = c.take<float>(rows * k);
+  r.sums = c.take<float>(rows * 6);
+  bytes = c.used;
+  return r;
+}
 
 }  // namespace
 
+size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V, int k) {
+  return carve_topk(rows * splits_of(type, z, rows, V, kTopVec * kThreads), k, nullptr).bytes;
+}
 cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float inv_t, int32_t* ids, float* lp,
-                         cudaStream_t stream) {
-  return by_type(type, [&](auto t) {
+                         void* workspace, cudaStream_t stream) {
+  const int splits = splits_of(type, z, rows, V, kTopVec * kThreads);
+  const TopWork w = carve_topk(rows * splits, k, workspace);
+  const int groups = k <= 24 ? 32 : k <= 48 ? 64 : k <= 96 ? 128 : 256;
+  Shape units, merge;
+  units.blocks = merge.blocks = rows;
+  units.units = splits;
+  merge.early = true;
+  const cudaError_t e = by_type(type, [&](auto t) {
     using T = decltype(t);
-    const Plan p = plan_of(rows, V, Vec<T>::N, 16);
-    const int groups = k <= 24 ? 32 : k <= 48 ? 64 : k <= 96 ? 128 : 256;
-    return launch(topk_kernel<T>, rows * p.cluster, kThreads, p.cluster, p.per * 16 + (p.cluster + 1) * k * 8, false,
-                  stream, static_cast<const T*>(z.p), z.ld, V, p.per, k, groups, kLog2e * inv_t, ids, lp);
+    return launch(topk_units_kernel<T>, units, stream, static_cast<const T*>(z.p), z.ld, rows, V, k, groups, kLog2e * inv_t,
+                  w.parts, w.lists);
   });
+  if (e != cudaSuccess) return e;
+  return launch(topk_merge_kernel, merge, stream, splits, k, groups, kLog2e * inv_t, w.parts, w.lists, ids, lp);
 }
 
-cudaError_t kd_topk(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight, float* loss,
-                    float* stats, void* out, int64_t out_ld, cudaStream_t stream) {
+size_t kd_topk_loss_workspace(Type type, Logits z, int64_t rows, int V) {
+  return rows * splits_of(type, z, rows, V, kPartVec * kThreads) * sizeof(unsigned long long);
+}
+cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, float* loss, float* stats,
+                         void* workspace, cudaStream_t stream) {
+  const int splits = splits_of(type, z, rows, V, kPartVec * kThreads);
+  unsigned long long* words = static_cast<unsigned long long*>(workspace);
+  Shape parts, last;
+  parts.blocks = last.blocks = rows;
+  parts.units = splits;
+  last.threads = 32;
+  last.early = true;
   return by_type(type, [&](auto x) {
     using T = decltype(x);
-    const Plan p = plan_of(rows, V, Vec<T>::N, 16);
-    return launch(out ? kd_kernel<T, true> : kd_kernel<T, false>, rows * p.cluster, kThreads, p.cluster, p.per * 16,
-                  false, stream, static_cast<const T*>(z.p), z.ld, V, p.per, t, kLog2e * inv_t, inv_t, weight, loss,
-                  reinterpret_cast<KdRow*>(stats), static_cast<T*>(out), out_ld);
+    const T* p = static_cast<const T*>(z.p);
+    const cudaError_t e = launch(kd_parts_kernel<T>, parts, stream, p, z.ld, rows, V, t, kLog2e * inv_t, words);
+    if (e != cudaSuccess) return e;
+    return launch(kd_loss_kernel<T>, last, stream, p, z.ld, splits, V, t, kLog2e * inv_t, words, loss,
+                  reinterpret_cast<KdRow*>(stats));
   });
 }
-
+size_t kd_topk_grad_workspace(int64_t rows, int k) {
+  size_t bytes;
+  carve_kd(rows, k, nullptr, bytes);
+  return bytes;
+}
+cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight,
+                         float* loss, void* out, int64_t out_ld, void* workspace, cudaStream_t stream) {
+  size_t bytes;
+  const KdRows r = carve_kd(rows, t.k, workspace, bytes);
+  const Plan p = plan_of(type, rows, V, 1);
+  Shape prepare, grad;
+  prepare.blocks = rows;
+  prepare.threads = 32;
+  grad.blocks = rows * p.cluster;
+  grad.threads = kRowThreads;
+  grad.cluster = p.cluster;
+  grad.smem = p.smem;
+  grad.early = true;
+  return by_type(type, [&](auto x) {
+    using T = decltype(x);
+    const T* src = static_cast<const T*>(z.p);
+    const cudaError_t e = launch(kd_prepare_kernel<T>, prepare, stream, src, z.ld, V, t, kLog2e * inv_t, inv_t, weight, r);
+    if (e != cudaSuccess) return e;
+    return launch(kd_grad_kernel<T>, grad, stream, src, z.ld, V, p.keep, t.k, kLog2e * inv_t, loss, static_cast<T*>(out),
+                  out_ld, r);
+  });
+}
 cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight,
                         const float* stats, void* out, int64_t out_ld, cudaStream_t stream) {
+  Shape s;
+  s.blocks = rows;
+  s.units = splits_of(type, z, rows, V, kKdVec * kThreads);
   return by_type(type, [&](auto x) {
     using T = decltype(x);
-    const int total = (V + Vec<T>::N - 1) / Vec<T>::N + 1, per = kBwdVectors * kThreads, splits = (total + per - 1) / per;
-    return launch(kd_bwd_kernel<T>, rows * splits, kThreads, 1, 0, false, stream, static_cast<const T*>(z.p), z.ld, V,
-                  per, splits, t, kLog2e * inv_t, inv_t, weight, reinterpret_cast<const KdRow*>(stats),
-                  static_cast<T*>(out), out_ld);
+    return launch(kd_bwd_kernel<T>, s, stream, static_cast<const T*>(z.p), z.ld, rows, V, t, kLog2e * inv_t, inv_t, weight,
+                  reinterpret_cast<const KdRow*>(stats), static_cast<T*>(out), out_ld);
   });
 }
 
 cudaError_t accept_kl(Type type, Logits draft, Logits target, int64_t rows, int V, float inv_t, float* alpha, float* kl,
                       float* stats, cudaStream_t stream) {
+  const Plan p = plan_of(type, rows, V, 2);
+  Shape s;
+  s.blocks = rows * p.cluster;
+  s.threads = kRowThreads;
+  s.cluster = p.cluster;
+  s.smem = p.smem;
   return by_type(type, [&](auto x) {
     using T = decltype(x);
-    const Plan p = plan_of(rows, V, Vec<T>::N, 32);
-    return launch(accept_kernel<T>, rows * p.cluster, kThreads, p.cluster, p.per * 32, false, stream,
-                  static_cast<const T*>(draft.p), draft.ld, static_cast<const T*>(target.p), target.ld, V, p.per,
-                  kLog2e * inv_t, alpha, kl, reinterpret_cast<AcceptRow*>(stats));
+    return launch(accept_kernel<T>, s, stream, static_cast<const T*>(draft.p), draft.ld, static_cast<const T*>(target.p),
+                  target.ld, V, p.keep, kLog2e * inv_t, alpha, kl, reinterpret_cast<AcceptRow*>(stats));
   });
 }
-
 cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, int V, float inv_t, const float* stats,
                           const float* g_alpha, const float* g_kl, void* out, int64_t out_ld, cudaStream_t stream) {
+  Shape s;
+  s.blocks = rows;
+  s.units = splits_of(type, draft, rows, V, kPairVec * kThreads);
   return by_type(type, [&](auto x) {
     using T = decltype(x);
-    const int total = (V + Vec<T>::N - 1) / Vec<T>::N + 1, per = kBwdVectors * kThreads, splits = (total + per - 1) / per;
-    return launch(accept_bwd_kernel<T>, rows * splits, kThreads, 1, 0, false, stream, static_cast<const T*>(draft.p),
-                  draft.ld, static_cast<const T*>(target.p), target.ld, V, per, splits, kLog2e * inv_t, inv_t,
+    return launch(accept_bwd_kernel<T>, s, stream, static_cast<const T*>(draft.p), draft.ld,
+                  static_cast<const T*>(target.p), target.ld, rows, V, kLog2e * inv_t, inv_t,
                   reinterpret_cast<const AcceptRow*>(stats), g_alpha, g_kl, static_cast<T*>(out), out_ld);
   });
 }
@@ -1157,13 +1782,19 @@ cudaError_t spec_verify(const Verify& a, cudaStream_t stream) {
   const VerifyPlan p = verify_plan(a);
   return by_type(a.type, [&](auto x) {
     using T = decltype(x);
-    cudaError_t e = launch(p.unroll == 8 ? verify_parts_kernel<T, 8> : verify_parts_kernel<T, 2>,
-                           a.batch * p.rows * p.splits, kThreads, 1, 0, false, stream, a, p.splits);
+    Shape parts, draw;
+    parts.blocks = a.batch * p.rows * p.splits;
+    cudaError_t e = launch(p.unroll == 8 ? verify_parts_kernel<T, 8> : verify_parts_kernel<T, 2>, parts, stream, a,
+                           p.splits);
     if (e != cudaSuccess) return e;
     const int total = (a.V + Vec<T>::N - 1) / Vec<T>::N + 1;
     int c = 1;
     while (c < kMaxCluster && total > kDrawThreads * c && (c < 8 || a.batch * c < sm_count())) c *= 2;
-    return launch(verify_draw_kernel<T>, a.batch * c, kDrawThreads, c, 0, true, stream, a, p.splits, (total + c - 1) / c);
+    draw.blocks = a.batch * c;
+    draw.threads = kDrawThreads;
+    draw.cluster = c;
+    draw.early = true;
+    return launch(verify_draw_kernel<T>, draw, stream, a, p.splits, (total + c - 1) / c);
   });
 }
 

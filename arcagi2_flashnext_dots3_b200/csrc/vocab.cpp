@@ -54,6 +54,9 @@ v::Type type_of(const torch::Tensor& t) {
   return t.scalar_type() == torch::kFloat ? v::F32 : t.scalar_type() == torch::kHalf ? v::F16 : v::BF16;
 }
 v::Logits rows_of(const torch::Tensor& t) { return {t.data_ptr(), t.stride(0)}; }
+torch::Tensor bytes_like(const torch::Tensor& t, size_t n) {
+  return torch::empty({(int64_t)n}, t.options().dtype(torch::kUInt8));
+}
 float* opt(const c10::optional<torch::Tensor>& t) { return t ? t->data_ptr<float>() : nullptr; }
 
 void teacher_topk(torch::Tensor logits, double temp, torch::Tensor ids, torch::Tensor lp) {
@@ -65,8 +68,10 @@ void teacher_topk(torch::Tensor logits, double temp, torch::Tensor ids, torch::T
   const float inv_t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(logits.device());
+  const torch::Tensor ws = bytes_like(logits, v::teacher_topk_workspace(type_of(logits), rows_of(logits), n, logits.size(1), k));
   launched(v::teacher_topk(type_of(logits), rows_of(logits), n, logits.size(1), k, inv_t, ids.data_ptr<int32_t>(),
-                           lp.data_ptr<float>(), at::cuda::getCurrentCUDAStream()), "teacher_topk");
+                           lp.data_ptr<float>(), ws.data_ptr(), at::cuda::getCurrentCUDAStream()),
+           "teacher_topk");
 }
 
 v::Teacher check_kd(const torch::Tensor& logits, const torch::Tensor& t_ids, const torch::Tensor& t_lp) {
@@ -76,23 +81,36 @@ v::Teacher check_kd(const torch::Tensor& logits, const torch::Tensor& t_ids, con
   check_vec(t_lp, logits, t_ids.numel(), torch::kFloat, "t_lp");
   return {t_ids.data_ptr(), wide, t_lp.data_ptr<float>(), (int)t_ids.size(1)};
 }
-// loss of each row; with weight and out also out = d sum(weight * loss) / d logits (out may be the logits themselves);
-// with stats what kd_topk_bwd needs.
-void kd_topk(torch::Tensor logits, torch::Tensor t_ids, torch::Tensor t_lp, double temp, torch::Tensor loss,
-             c10::optional<torch::Tensor> stats, c10::optional<torch::Tensor> weight, c10::optional<torch::Tensor> out) {
+// loss of each row; with stats what kd_topk_bwd needs
+void kd_topk_loss(torch::Tensor logits, torch::Tensor t_ids, torch::Tensor t_lp, double temp, torch::Tensor loss,
+                  c10::optional<torch::Tensor> stats) {
   const v::Teacher teacher = check_kd(logits, t_ids, t_lp);
   const int64_t n = logits.size(0);
   check_vec(loss, logits, n, torch::kFloat, "loss");
   if (stats) check_vec(*stats, logits, n * v::kKdStats, torch::kFloat, "stats");
-  TORCH_CHECK(weight.has_value() == out.has_value(), "the gradient form takes weight and out together");
-  if (weight) check_vec(*weight, logits, n, torch::kFloat, "weight");
-  if (out) check_out(*out, logits, "out");
   const float inv_t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(logits.device());
-  launched(v::kd_topk(type_of(logits), rows_of(logits), n, logits.size(1), teacher, inv_t, opt(weight),
-                      loss.data_ptr<float>(), opt(stats), out ? out->data_ptr() : nullptr, out ? out->stride(0) : 0,
-                      at::cuda::getCurrentCUDAStream()), "kd_topk");
+  const torch::Tensor ws = bytes_like(logits, v::kd_topk_loss_workspace(type_of(logits), rows_of(logits), n, logits.size(1)));
+  launched(v::kd_topk_loss(type_of(logits), rows_of(logits), n, logits.size(1), teacher, inv_t, loss.data_ptr<float>(),
+                           opt(stats), ws.data_ptr(), at::cuda::getCurrentCUDAStream()), "kd_topk_loss");
+}
+
+// loss of each row and out = d sum(weight * loss) / d logits; out may be the logits themselves
+void kd_topk_grad(torch::Tensor logits, torch::Tensor t_ids, torch::Tensor t_lp, double temp, torch::Tensor weight,
+                  torch::Tensor loss, torch::Tensor out) {
+  const v::Teacher teacher = check_kd(logits, t_ids, t_lp);
+  const int64_t n = logits.size(0);
+  check_vec(loss, logits, n, torch::kFloat, "loss");
+  check_vec(weight, logits, n, torch::kFloat, "weight");
+  check_out(out, logits, "out");
+  const float inv_t = check_temp(temp);
+  if (!n) return;
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const torch::Tensor ws = bytes_like(logits, v::kd_topk_grad_workspace(n, teacher.k));
+  launched(v::kd_topk_grad(type_of(logits), rows_of(logits), n, logits.size(1), teacher, inv_t, weight.data_ptr<float>(),
+                           loss.data_ptr<float>(), out.data_ptr(), out.stride(0), ws.data_ptr(),
+                           at::cuda::getCurrentCUDAStream()), "kd_topk_grad");
 }
 
 void kd_topk_bwd(torch::Tensor logits, torch::Tensor t_ids, torch::Tensor t_lp, double temp, torch::Tensor stats,
@@ -191,7 +209,7 @@ void spec_verify(torch::Tensor logits, torch::Tensor drafts, torch::Tensor temps
   a.n_draft = n_draft ? n_draft->data_ptr<int32_t>() : nullptr;
   a.accepted = accepted.data_ptr<int32_t>();
   a.next = next.data_ptr<int32_t>();
-  const torch::Tensor ws = torch::empty({(int64_t)v::spec_verify_workspace(a)}, logits.options().dtype(torch::kUInt8));
+  const torch::Tensor ws = bytes_like(logits, v::spec_verify_workspace(a));
   a.workspace = ws.data_ptr();
   launched(v::spec_verify(a, at::cuda::getCurrentCUDAStream()), "spec_verify");
 }
@@ -200,7 +218,8 @@ void spec_verify(torch::Tensor logits, torch::Tensor drafts, torch::Tensor temps
 
 void register_vocab(pybind11::module& m) {
   m.def("teacher_topk", &teacher_topk);
-  m.def("kd_topk", &kd_topk);
+  m.def("kd_topk_loss", &kd_topk_loss);
+  m.def("kd_topk_grad", &kd_topk_grad);
   m.def("kd_topk_bwd", &kd_topk_bwd);
   m.def("accept_kl", &accept_kl);
   m.def("accept_kl_bwd", &accept_kl_bwd);

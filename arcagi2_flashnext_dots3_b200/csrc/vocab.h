@@ -10,7 +10,7 @@ namespace vocab {
 enum Type { F32 = 0, F16 = 1, BF16 = 2 };
 
 constexpr int kMaxK = 128;       // teacher tokens per row, drafts per sequence
-constexpr int kMaxV = 400000;    // both rows of accept_kl in fp32 fit the shared memory of a 16-CTA cluster
+constexpr int kMaxV = 1 << 20;
 constexpr int kKdStats = 4;      // floats of per-row state between kd_topk and kd_topk_bwd
 constexpr int kAcceptStats = 5;  // floats of per-row state between accept_kl and accept_kl_bwd
 
@@ -26,12 +26,19 @@ struct Teacher {                 // [rows, k] ids (int32 or int64) and fp32 log-
   int k;
 };
 
+// A workspace has the bytes that its ..._workspace() says.
+size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V, int k);
 cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float inv_t, int32_t* ids, float* lp,
-                         cudaStream_t stream);
+                         void* workspace, cudaStream_t stream);
 
-// out == nullptr: loss only. stats may be null.
-cudaError_t kd_topk(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight, float* loss,
-                    float* stats, void* out, int64_t out_ld, cudaStream_t stream);
+// stats may be null
+size_t kd_topk_loss_workspace(Type type, Logits z, int64_t rows, int V);
+cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, float* loss, float* stats,
+                         void* workspace, cudaStream_t stream);
+// loss, and out = d sum(weight loss) / d logits; out may be the logits
+size_t kd_topk_grad_workspace(int64_t rows, int k);
+cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight,
+                         float* loss, void* out, int64_t out_ld, void* workspace, cudaStream_t stream);
 cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight,
                         const float* stats, void* out, int64_t out_ld, cudaStream_t stream);
 

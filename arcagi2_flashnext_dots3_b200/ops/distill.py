@@ -9,7 +9,7 @@ flashnext/training/draft_head/train.py); its code works in torch on whole [rows,
 * :func:`accept_kl` - sum min(q, p) and KL(p || q) of a draft distribution q against a target p, differentiable in
   the draft.
 
-Logits are [rows, vocab] in fp32, fp16 or bf16 (vocab up to 400000; rows may be strided). A logit at or below -1e30
+Logits are [rows, vocab] in fp32, fp16 or bf16 (vocab up to 393216; rows may be strided). A logit at or below -1e30
 (-inf, the lowest fp32 / bf16 value) is masked and has probability 0; a row with nothing left gives loss 0, gradient
 0 and id -1. A NaN makes its row's results NaN. Results per row are fp32, gradients have the logits' type. Nothing
 here reads from the host, so every call can be captured in a CUDA graph.
@@ -126,7 +126,7 @@ class _KDTopK(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             stats = torch.empty(n, 4, dtype=torch.float32, device=logits.device)
             ctx.save_for_backward(logits, t_ids, t_lp, stats)
-        native.C().kd_topk(logits, t_ids, t_lp, t, loss, stats, None, None)
+        native.C().kd_topk_loss(logits, t_ids, t_lp, t, loss, stats)
         return loss
 
     @staticmethod
@@ -169,7 +169,7 @@ def kd_topk_grad(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, 
         raise ValueError("out must have the logits' shape, type and device and unit stride along the vocabulary")
     if logits.is_cuda:
         loss = torch.empty(n, dtype=torch.float32, device=logits.device)
-        native.C().kd_topk(logits, t_ids, t_lp, t, loss, None, weight, out)
+        native.C().kd_topk_grad(logits, t_ids, t_lp, t, weight, loss, out)
         return loss, out
     loss, g = _kd_cpu(logits, t_ids, t_lp, t, weight)
     return loss, out.copy_(g)
