@@ -12,7 +12,7 @@
 //                  outside the K, not taken as 1 - sum ps: a confident student would lose it to cancellation.
 //   accept_kl    : q = softmax(draft / T), p = softmax(target / T): alpha = sum_v min(q_v, p_v) (the probability that
 //                  a token drawn from q is accepted), kl = KL(p || q);
-//                    d alpha / d zq_v = q_v ([q_v <= p_v] - A) / T, A = sum_v q_v [q_v <= p_v]
+//                    d alpha / d zq_v = q_v (h_v - A) / T, A = sum_v q_v h_v, h = 1 where q < p, 1/2 where q = p, else 0
 //                    d kl / d zq_v = (q_v - p_v) / T
 //   spec_verify  : draft j of a sequence is accepted while u q_j(d) < p_j(d); at the first rejection the next token
 //                  is drawn from the residual max(p - q, 0) (a point-mass draft: p without d), after the last draft
@@ -59,7 +59,9 @@ constexpr int kRowBlocks = 5;       // their blocks per SM
 constexpr int kKeep = 2560;          // vectors of a block that shared memory keeps (40 KB)
 constexpr float kTailFloor = 1e-8f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2ed = 1.4426950408889634;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr double kLn2d = 0.6931471805599453;
 // Smallest logit that is not masked, the float after -1e30, and the start of every running maximum: a masked logit's
 // ex2 argument against it (or anything above) is hugely negative, so masked logits add exactly 0 and no test is needed.
 constexpr float kFloor = -9.9999994e29f;
@@ -716,8 +718,7 @@ __device__ __forceinline__ void load_ids(const Teacher& t, int64_t row, int V, i
 
 // A row's teacher entries over the lanes of a warp.
 struct TeacherRow {
-  float lp[kE], pt[kE], z[kE];       // log-probability, probability, student logit (-inf and 0 where left out)
-  float tt;
+  float lp[kE], pt[kE], z[kE];       // log-probability, probability, student logit (-inf, 0 and -inf where left out)
   unsigned kept;                     // bit i: entry lane + 32 i is in the vocabulary and not repeated
 };
 template <typename T>
@@ -737,7 +738,6 @@ __device__ __forceinline__ TeacherRow teacher_row(int k, const int (&id)[kE], co
 #pragma unroll
   for (int i = 0; i < kE; ++i) s_id[lane + 32 * i] = id[i];
   __syncwarp();
-  double mass = 0.0;
   e.kept = 0;
 #pragma unroll
   for (int i = 0; i < kE; ++i) {
@@ -749,20 +749,19 @@ __device__ __forceinline__ TeacherRow teacher_row(int k, const int (&id)[kE], co
         e.z[i] = masked(z[i]);
         e.kept |= 1u << i;
       }
-      const double p = exp((double)e.lp[i]);
-      e.pt[i] = (float)p;
-      mass += p;
+      e.pt[i] = expf(e.lp[i]);
     }
   }
-  e.tt = (float)fmax(1.0 - warp_reduce(mass, Add()), (double)kTailFloor);   // a difference from 1: fp64
   __syncwarp();
   return e;
 }
 
-// What does not depend on the tail: offset and sum of the teacher's tokens' softmax, sum pt (log pt - log-offset terms), sum
-// pt, tt.
+// What does not depend on the tail: offset and sum of the softmax of the teacher's tokens, sum pt (log pt - log of their
+// terms), sum pt, tt and its logarithm. Losses can be small differences of these (a flat teacher leaves nearly all mass in
+// the tail), so what only they need is fp64.
 struct TeacherSums {
-  float c, es, l, mass, tt;
+  double l, mass, log_tt;
+  float c, es, tt, w;                  // w: the row's weight / T
 };
 __device__ __forceinline__ TeacherSums teacher_sums(const TeacherRow& e, float kl, int k) {
   TeacherSums r;
@@ -770,35 +769,43 @@ __device__ __forceinline__ TeacherSums teacher_sums(const TeacherRow& e, float k
 #pragma unroll
   for (int i = 0; i < kE; ++i) zm = fmaxf(zm, e.z[i]);
   r.c = warp_reduce(zm, Max()) * kl;
-  r.es = r.l = r.mass = 0.f;
+  r.es = 0.f;
+  r.l = r.mass = 0.0;
 #pragma unroll
   for (int i = 0; i < kE; ++i)
     if (32 * i < k) {
-      const float x = fmaf(e.z[i], kl, -r.c);
-      r.es += ex2(x);
-      if (e.pt[i] != 0.f) r.l += e.pt[i] * (e.lp[i] - kLn2 * x);
-      r.mass += e.pt[i];
+      const double pt = exp((double)e.lp[i]);
+      r.es += ex2(fmaf(e.z[i], kl, -r.c));
+      if (pt != 0.0) r.l += pt * ((double)e.lp[i] - kLn2d * ((double)e.z[i] * kl - r.c));
+      r.mass += pt;
     }
   r.es = warp_reduce(r.es, Add());
   r.l = warp_reduce(r.l, Add());
   r.mass = warp_reduce(r.mass, Add());
-  r.tt = e.tt;
+  const bool floor = 1.0 - r.mass < (double)kTailFloor;
+  r.tt = floor ? kTailFloor : (float)(1.0 - r.mass);
+  r.log_tt = floor ? log((double)kTailFloor) : log1p(-r.mass);
+  r.w = 0.f;
   return r;
 }
-// Statistics and loss of a row from its tail, the softmax of all but the teacher's tokens: with ps_k = p(id_k),
-// loss = sum pt (log pt - log ps) + tt (log tt - log ts).
-__device__ __forceinline__ KdRow kd_finish(const TeacherSums& e, const Soft& tail, float& loss) {
+// Statistics of a row from its tail, the softmax of all but the teacher's tokens.
+__device__ __forceinline__ KdRow kd_finish(const TeacherSums& e, const Soft& tail) {
   const float c = fmaxf(tail.c, e.c);
   const float tail_sum = tail.sum * ex2(tail.c - c), es = e.es * ex2(e.c - c), total = tail_sum + es;
-  if (total == 0.f) {                  // nothing in the row
-    loss = 0.f;
-    return KdRow{0.f, 0.f, 0.f, 0.f};
-  }
-  const float inv_s = 1.f / total, ts_raw = tail_sum * inv_s;
-  const float ts = ts_raw < kTailFloor ? kTailFloor : ts_raw, ratio = ts_raw < kTailFloor ? 0.f : e.tt / ts;
-  loss = e.l + e.tt * (logf(e.tt) - logf(ts));
-  if (e.mass != 0.f) loss += e.mass * kLn2 * ((c - e.c) + log2f(total));
-  return KdRow{c, inv_s, ratio, ratio * (es * inv_s) - e.mass};
+  if (total == 0.f) return KdRow{0.f, 0.f, 0.f, 0.f};      // nothing in the row
+  const float inv_s = 1.f / total, ts = tail_sum * inv_s, ratio = ts < kTailFloor ? 0.f : e.tt / ts;
+  return KdRow{c, inv_s, ratio, ratio * (es * inv_s) - (float)e.mass};
+}
+// sum pt (log pt - log ps) + tt (log tt - log ts); log ts = -log1p(teacher's / tail's sum) keeps its digits near ts = 1
+__device__ __forceinline__ float kd_loss(const TeacherSums& e, const Soft& tail) {
+  const float c = fmaxf(tail.c, e.c);
+  const float tail_sum = tail.sum * ex2(tail.c - c), es = e.es * ex2(e.c - c);
+  const double total = (double)tail_sum + es;
+  if (total == 0.0) return 0.f;
+  const double log_ts = tail_sum < kTailFloor * total ? log((double)kTailFloor) : -log1p((double)es / tail_sum);
+  double l = e.l + e.tt * (e.log_tt - log_ts);
+  if (e.mass != 0.0) l += e.mass * kLn2d * ((double)c - e.c + log2(total));
+  return (float)l;
 }
 // w d loss / d z at a teacher's token
 __device__ __forceinline__ float kd_pull(const KdRow& r, float w, float z, float pt, float kl) {
@@ -890,11 +897,9 @@ __global__ void __launch_bounds__(32) kd_loss_kernel(const T* logits, int64_t ld
   const TeacherSums sums = teacher_sums(teacher_row(t.k, id, lp, z, s_id), kl, t.k);
   pdl_wait();
   const Soft tail = join_parts(splits, kl, [&](int i) { return parts[row * splits + i]; });
-  float l;
-  const KdRow r = kd_finish(sums, tail, l);
   if (threadIdx.x == 0) {
-    loss[row] = l;
-    if (stats) stats[row] = r;
+    loss[row] = kd_loss(sums, tail);
+    if (stats) stats[row] = kd_finish(sums, tail);
   }
 }
 
@@ -903,7 +908,7 @@ __global__ void __launch_bounds__(32) kd_loss_kernel(const T* logits, int64_t ld
 struct KdRows {
   int* id;                           // [rows, k], -1: left out
   float *z, *pt;                     // [rows, k]
-  float* sums;                       // [rows, 6] TeacherSums, weight / T
+  TeacherSums* sums;                 // [rows]
 };
 template <typename T>
 __global__ void __launch_bounds__(32) kd_prepare_kernel(const T* logits, int64_t ld, int V, Teacher t, float kl, float inv_t,
@@ -925,16 +930,9 @@ __global__ void __launch_bounds__(32) kd_prepare_kernel(const T* logits, int64_t
       r.z[at] = e.z[i];
       r.pt[at] = e.pt[i];
     }
-  const TeacherSums s = teacher_sums(e, kl, t.k);
-  if (lane == 0) {
-    float* o = r.sums + 6 * row;
-    o[0] = s.c;
-    o[1] = s.es;
-    o[2] = s.l;
-    o[3] = s.mass;
-    o[4] = s.tt;
-    o[5] = weight[row] * inv_t;
-  }
+  TeacherSums s = teacher_sums(e, kl, t.k);
+  s.w = weight[row] * inv_t;
+  if (lane == 0) r.sums[row] = s;
 }
 
 // The teacher's tokens in a block's share of a row.
@@ -1032,11 +1030,10 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) kd_grad_kernel(const 
   }
   cluster_sync();
   const Soft tail = join_parts(size, kl, [&](int i) { return part[i]; });
-  const float* sums = r.sums + 6 * row;
-  const float w = sums[5];
-  float l;
-  const KdRow f = kd_finish(TeacherSums{sums[0], sums[1], sums[2], sums[3], sums[4]}, tail, l);
-  if (rank == 0 && tid == 0) loss[row] = l;
+  const TeacherSums& e = r.sums[row];
+  const KdRow f = kd_finish(e, tail);
+  const float w = e.w;
+  if (rank == 0 && tid == 0) loss[row] = kd_loss(e, tail);
   T* o = out + row * out_ld;
   const Two scale = two(f.inv_s == 0.f ? 0.f : -f.csum * f.inv_s * w), c2 = two(-f.c), k2 = two(kl);
   if (same_phase<T>(o, s.row)) {
@@ -1088,66 +1085,66 @@ __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64
   if (id >= 0 && s.place(id) >= 0) {
     bool repeated = false;
     for (int j = 0; j < tid; ++j) repeated |= load_id(t, row * t.k + j, V) == id;
-    const float pt = (float)exp((double)t.lp[row * t.k + tid]);
+    const float pt = expf(t.lp[row * t.k + tid]);
     if (!repeated) o[id] = Vec<T>::back(kd_pull(st, w, masked(Vec<T>::one(s.row[id])), pt, kl));
   }
 }
 
 // ------------------------------------------------------------------------------------------- acceptance and KL
 // log2 q_v = zq_v kl - bq up to the rounding of bq, whose remainder is in fq = 2^(rounded - exact), and for p alike; a =
-// sum_v q_v [q_v <= p_v]. fq = 0 marks a row with nothing to compare.
+// sum_v q_v h_v. fq = 0 marks a row with nothing to compare. mq, lq, mp, lp: maxima (divided by T) and log-sums, from which
+// the gradient forms the log-probabilities that it compares.
 struct AcceptRow {
-  float bq, fq, bp, fp, a;
+  float bq, fq, bp, fp, a, mq, lq, mp, lp;
 };
 static_assert(sizeof(AcceptRow) == kAcceptStats * 4, "AcceptRow is what callers allocate");
 
-// Both softmaxes and d = sum 2^xp (xp - xq) with xq, xp the ex2 arguments of the elements: KL in bits is then
-// d / sum_p + log2 sum_q - log2 sum_p, and no second pass needs the probabilities of p.
+// Both softmaxes, with their largest logits in place of the offsets, and d = sum 2^xp (xp - xq) with xq, xp the ex2 arguments
+// of the elements: KL in bits is then d / sum_p + log2 sum_q - log2 sum_p, and no second look needs the probabilities of p.
 struct Pair {
-  Soft q, p;
-  float d;
+  float mq, sq, mp, sp, d;
 };
-__device__ __forceinline__ Pair join(const Pair& a, const Pair& b) {
+// The rounded offset of a maximum: never contracted into an FMA, or its uses would differ.
+__device__ __forceinline__ float offset(float m, float kl) { return __fmul_rn(m, kl); }
+__device__ __forceinline__ Pair join(const Pair& a, const Pair& b, float kl) {
   Pair r;
-  r.q = join(a.q, b.q);
-  r.p.c = fmaxf(a.p.c, b.p.c);
-  const float ea = ex2(a.p.c - r.p.c), eb = ex2(b.p.c - r.p.c);
-  r.p.sum = a.p.sum * ea + b.p.sum * eb;
+  r.mq = fmaxf(a.mq, b.mq);
+  r.mp = fmaxf(a.mp, b.mp);
+  const float cq = offset(r.mq, kl), cp = offset(r.mp, kl);
+  const float qa = offset(a.mq, kl) - cq, qb = offset(b.mq, kl) - cq, pa = offset(a.mp, kl) - cp, pb = offset(b.mp, kl) - cp;
+  const float ea = ex2(pa), eb = ex2(pb);
+  r.sq = a.sq * ex2(qa) + b.sq * ex2(qb);
+  r.sp = a.sp * ea + b.sp * eb;
   // the arguments move by the change of their offsets; a part whose weight vanishes adds nothing, even if infinite
-  const float da = a.d + a.p.sum * ((a.p.c - r.p.c) - (a.q.c - r.q.c));
-  const float db = b.d + b.p.sum * ((b.p.c - r.p.c) - (b.q.c - r.q.c));
+  const float da = a.d + a.sp * (pa - qa), db = b.d + b.sp * (pb - qb);
   r.d = (ea == 0.f ? 0.f : ea * da) + (eb == 0.f ? 0.f : eb * db);
   return r;
 }
 __device__ __forceinline__ Pair shfl_xor(const Pair& a, int o) {
-  return {shfl_xor(a.q, o), shfl_xor(a.p, o), __shfl_xor_sync(0xffffffffu, a.d, o)};
+  const auto x = [&](float f) { return __shfl_xor_sync(0xffffffffu, f, o); };
+  return {x(a.mq), x(a.sq), x(a.mp), x(a.sp), x(a.d)};
 }
 
 constexpr int kPairVec = 4;          // vectors per thread, unit and side of the gradient
 
 template <typename Load>
 __device__ __forceinline__ Pair join_pairs(int n, float kl, Load load) {
-  Pair t{{kFloor * kl, 0.f}, {kFloor * kl, 0.f}, 0.f};
-  for (int i = threadIdx.x & 31; i < n; i += 32) t = join(t, load(i));
+  Pair t{kFloor, 0.f, kFloor, 0.f, 0.f};
+  for (int i = threadIdx.x & 31; i < n; i += 32) t = join(t, load(i), kl);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) t = join(t, shfl_xor(t, o));
+  for (int o = 16; o; o >>= 1) t = join(t, shfl_xor(t, o), kl);
   return t;
 }
-// Adds pairs of vectors to a thread's running Pair with maxima mq, mp.
+// Adds pairs of vectors to a thread's running Pair.
 template <typename T, int kVec>
-__device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&xp)[kVec], float kl, float& mq, float& mp,
-                                         Pair& a) {
+__device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&xp)[kVec], float kl, Pair& a) {
   constexpr int N = Vec<T>::N;
   const float vq = unit_max<T>(xq), vp = unit_max<T>(xp);
   float low = packed_min<T>(xq[0]);
 #pragma unroll
   for (int i = 0; i < kVec; ++i) low = fminf(low, fminf(packed_min<T>(xq[i]), packed_min<T>(xp[i])));
-  if (vq > mq || vp > mp) {
-    mq = fmaxf(mq, vq);
-    mp = fmaxf(mp, vp);
-    a = join(a, Pair{{mq * kl, 0.f}, {mp * kl, 0.f}, 0.f});
-  }
-  const Two k2 = two(kl), cq = two(-a.q.c), cp = two(-a.p.c), minus = two(-1.f);
+  if (vq > a.mq || vp > a.mp) a = join(a, Pair{fmaxf(vq, kFloor), 0.f, fmaxf(vp, kFloor), 0.f, 0.f}, kl);
+  const Two k2 = two(kl), cq = two(-offset(a.mq, kl)), cp = two(-offset(a.mp, kl)), minus = two(-1.f);
   Two sq = two(0.f), sp = two(0.f), d = two(0.f);
   const auto look = [&](auto guarded) {
 #pragma unroll
@@ -1177,15 +1174,15 @@ __device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&
   // masked logits: 0 times an infinite gap is 0, and a token that only the draft masks makes KL infinite, whatever masks it
   if (low >= kFloor) look(std::false_type());
   else look(std::true_type());
-  a.q.sum += sum(sq);
-  a.p.sum += sum(sp);
+  a.sq += sum(sq);
+  a.sp += sum(sp);
   a.d += sum(d);
 }
 
 // One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p).
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, kRowBlocks) accept_kernel(const T* draft, int64_t ldq, const T* target,
-                                                                         int64_t ldp, int V, int keep, float kl,
+                                                                         int64_t ldp, int V, int keep, float kl, float temp,
                                                                          float* alpha, float* out_kl, AcceptRow* stats) {
   constexpr int N = Vec<T>::N;
   extern __shared__ uint4 dyn[];
@@ -1209,36 +1206,38 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) accept_kernel(const T
     *reinterpret_cast<T*>(lone[0]) = s.row[single];
     *reinterpret_cast<T*>(lone[1]) = other[single];
   }
-  float mq = kFloor, mp = kFloor;
-  Pair a{{kFloor * kl, 0.f}, {kFloor * kl, 0.f}, 0.f};
+  Pair a{kFloor, 0.f, kFloor, 0.f, 0.f};
   for (int v = s.kept + tid; v < s.n; v += 2 * kRowThreads) {
     uint4 xq[2], xp[2];
     stream(s, s.row, true, v, xq);
     stream(s, other, same, v, xp);
-    add_pair<T>(xq, xp, kl, mq, mp, a);
+    add_pair<T>(xq, xp, kl, a);
   }
-  if (single >= 0) add_pair<T>(lone[0], lone[1], kl, mq, mp, a);
+  if (single >= 0) add_pair<T>(lone[0], lone[1], kl, a);
   wait_copies();
   for (int v = tid; v < s.kept; v += 2 * kRowThreads) {
     const uint4 xq[2] = {dq[v], dq[v + kRowThreads]}, xp[2] = {dp[v], dp[v + kRowThreads]};
-    add_pair<T>(xq, xp, kl, mq, mp, a);
+    add_pair<T>(xq, xp, kl, a);
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) a = join(a, shfl_xor(a, o));
+  for (int o = 16; o; o >>= 1) a = join(a, shfl_xor(a, o), kl);
   if (lane == 0) warp_pair[tid >> 5] = a;
   __syncthreads();
   cluster_peers_run();
   if (tid < 32) {
     a = join_pairs(kRowWarps, kl, [&](int i) { return warp_pair[i]; });
     if (lane < (int)size) {
-      st_peer(&part[0][rank], lane, as_u64(a.q.c, a.q.sum));
-      st_peer(&part[1][rank], lane, as_u64(a.p.c, a.p.sum));
+      st_peer(&part[0][rank], lane, as_u64(a.mq, a.sq));
+      st_peer(&part[1][rank], lane, as_u64(a.mp, a.sp));
       st_peer(&part[2][rank], lane, as_u64(a.d, 0.f));
     }
   }
   cluster_sync();
-  a = join_pairs(size, kl, [&](int i) { return Pair{as_soft(part[0][i]), as_soft(part[1][i]), as_soft(part[2][i]).c}; });
-  const float rq = a.q.c + log2f(a.q.sum), rp = a.p.c + log2f(a.p.sum);
+  a = join_pairs(size, kl, [&](int i) {
+    const Soft q = as_soft(part[0][i]), p = as_soft(part[1][i]);
+    return Pair{q.c, q.sum, p.c, p.sum, as_soft(part[2][i]).c};
+  });
+  const float cq = offset(a.mq, kl), cp = offset(a.mp, kl), rq = cq + log2f(a.sq), rp = cp + log2f(a.sp);
   float under = 0.f, over = 0.f;             // sums of min(q, p) where q <= p and where q > p
   const Two k2 = two(kl), bq = two(-rq), bp = two(-rp);
   const auto look = [&](const uint4& uq, const uint4& up) {
@@ -1282,18 +1281,26 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) accept_kernel(const T
     x += as_soft(sums[i]).c;
     y += as_soft(sums[i]).sum;
   }
-  const double lq = log2((double)a.q.sum), lp = log2((double)a.p.sum);
-  const float fq = exp2f((float)((double)rq - (a.q.c + lq))), fp = exp2f((float)((double)rp - (a.p.c + lp)));
-  const bool nothing = a.q.sum == 0.f || a.p.sum == 0.f;
-  const bool nan = isnan(a.q.sum) || isnan(a.p.sum);      // the minimum drops a NaN operand
+  const double lq = log2((double)a.sq), lp = log2((double)a.sp);
+  const float fq = exp2f((float)((double)rq - (cq + lq))), fp = exp2f((float)((double)rp - (cp + lp)));
+  const bool nothing = a.sq == 0.f || a.sp == 0.f;
+  const bool nan = isnan(a.sq) || isnan(a.sp);            // the minimum drops a NaN operand
   alpha[row] = nothing ? 0.f : nan ? NAN : fq * x + fp * y;
-  out_kl[row] = nothing ? 0.f : (float)((double)kLn2 * ((double)a.d / a.p.sum + lq - lp));
-  if (stats) stats[row] = nothing ? AcceptRow{0.f, 0.f, 0.f, 0.f, 0.f} : AcceptRow{rq, fq, rp, fp, fq * x};
+  out_kl[row] = nothing ? 0.f : (float)(kLn2d * ((double)a.d / a.sp + lq - lp));
+  if (!stats) return;
+  const float mq = a.mq / temp, mp = a.mp / temp;
+  // natural log of sum exp((z - m) / T): the offsets' roundings taken back
+  const float log_q = (float)(kLn2d * (lq + ((double)cq - (double)a.mq * kl)));
+  const float log_p = (float)(kLn2d * (lp + ((double)cp - (double)a.mp * kl)));
+  stats[row] = nothing ? AcceptRow{} : AcceptRow{rq, fq, rp, fp, fq * x, mq, log_q, mp, log_p};
 }
 
+// Which of q_v, p_v is smaller decides a jump of the gradient, so the comparison is not left to the ex2 arguments, whose
+// rounded offsets are off by up to 2^-20: log-probabilities are formed as a log-softmax forms them, ((z / T) - max) - log
+// sum, each step rounded to fp32. Equal ones take the mean of the two sides.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, int64_t ldq, const T* target, int64_t ldp,
-                                                              int64_t rows, int V, float kl, float inv_t,
+                                                              int64_t rows, int V, float kl, float temp,
                                                               const AcceptRow* stats, const float* g_alpha,
                                                               const float* g_kl, T* out, int64_t out_ld) {
   constexpr int N = Vec<T>::N;
@@ -1305,24 +1312,33 @@ __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, in
   load_unit(s, target + row * ldp, 0, xp);
   const AcceptRow st = stats[row];
   const bool nothing = st.fq == 0.f;
-  const float ga = g_alpha[row] * inv_t, gk = g_kl[row] * inv_t;
-  const float under = st.fq * (ga * (1.f - st.a) + gk), over = st.fq * (gk - ga * st.a);
+  const float ga = g_alpha[row] / temp, gk = g_kl[row] / temp;
+  const float under = st.fq * (ga * (1.f - st.a) + gk), over = st.fq * (gk - ga * st.a), even = 0.5f * (under + over);
   const Two k2 = two(kl), bq = two(-st.bq), bp = two(-st.bp), kp = two(-gk * st.fp);
-  store_unit<kPairVec>(s, out + row * out_ld, [&](int i) {
-    float q[N], p[N];
-    Vec<T>::unpack(xq[i], q);
-    Vec<T>::unpack(xp[i], p);
+  const auto unit = [&](auto cold) {
+    store_unit<kPairVec>(s, out + row * out_ld, [&](int i) {
+      float q[N], p[N];
+      Vec<T>::unpack(xq[i], q);
+      Vec<T>::unpack(xp[i], p);
 #pragma unroll
-    for (int k = 0; k < N; k += 2) {
-      const Two eq = fma2(two(q[k], q[k + 1]), k2, bq), ep = fma2(two(p[k], p[k + 1]), k2, bp);
-      const float2 fq = halves(eq), fp = halves(ep);
-      const float2 g = halves(fma2(ex2_two(eq), two(fq.x <= fp.x ? under : over, fq.y <= fp.y ? under : over),
-                                   mul2(kp, ex2_two(ep))));
-      q[k] = nothing ? 0.f : g.x;
-      q[k + 1] = nothing ? 0.f : g.y;
-    }
-    return Vec<T>::pack(q);
-  });
+      for (int k = 0; k < N; k += 2) {
+        float side[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float zq = cold ? __fdiv_rn(q[k + j], temp) : q[k + j], zp = cold ? __fdiv_rn(p[k + j], temp) : p[k + j];
+          const float lq = __fsub_rn(__fsub_rn(zq, st.mq), st.lq), lp = __fsub_rn(__fsub_rn(zp, st.mp), st.lp);
+          side[j] = lq < lp ? under : lq == lp ? even : over;
+        }
+        const Two eq = fma2(two(q[k], q[k + 1]), k2, bq), ep = fma2(two(p[k], p[k + 1]), k2, bp);
+        const float2 g = halves(fma2(ex2_two(eq), two(side[0], side[1]), mul2(kp, ex2_two(ep))));
+        q[k] = nothing ? 0.f : g.x;
+        q[k + 1] = nothing ? 0.f : g.y;
+      }
+      return Vec<T>::pack(q);
+    });
+  };
+  if (temp == 1.f) unit(std::false_type());
+  else unit(std::true_type());
 }
 
 // ------------------------------------------------------------------------------------------- draft verification
@@ -1645,7 +1661,7 @@ KdRows carve_kd(int64_t rows, int k, void* p, size_t& bytes) {
   r.id = c.take<int>(rows * k);
   r.z = c.take<float>(rows * k);
   r.pt = c.take<float>(rows * k);
-  r.sums = c.take<float>(rows * 6);
+  r.sums = c.take<TeacherSums>(rows);
   bytes = c.used;
   return r;
 }
@@ -1655,7 +1671,7 @@ KdRows carve_kd(int64_t rows, int k, void* p, size_t& bytes) {
 size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V, int k) {
   return carve_topk(rows * splits_of(type, z, rows, V, kTopVec * kThreads), k, nullptr).bytes;
 }
-cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float inv_t, int32_t* ids, float* lp,
+cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float temp, int32_t* ids, float* lp,
                          void* workspace, cudaStream_t stream) {
   const int splits = splits_of(type, z, rows, V, kTopVec * kThreads);
   const TopWork w = carve_topk(rows * splits, k, workspace);
@@ -1666,17 +1682,17 @@ cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float 
   merge.early = true;
   const cudaError_t e = by_type(type, [&](auto t) {
     using T = decltype(t);
-    return launch(topk_units_kernel<T>, units, stream, static_cast<const T*>(z.p), z.ld, rows, V, k, groups, kLog2e * inv_t,
+    return launch(topk_units_kernel<T>, units, stream, static_cast<const T*>(z.p), z.ld, rows, V, k, groups, (float)(kLog2ed / temp),
                   w.parts, w.lists);
   });
   if (e != cudaSuccess) return e;
-  return launch(topk_merge_kernel, merge, stream, splits, k, groups, kLog2e * inv_t, w.parts, w.lists, ids, lp);
+  return launch(topk_merge_kernel, merge, stream, splits, k, groups, (float)(kLog2ed / temp), w.parts, w.lists, ids, lp);
 }
 
 size_t kd_topk_loss_workspace(Type type, Logits z, int64_t rows, int V) {
   return rows * splits_of(type, z, rows, V, kPartVec * kThreads) * sizeof(unsigned long long);
 }
-cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, float* loss, float* stats,
+cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, float* loss, float* stats,
                          void* workspace, cudaStream_t stream) {
   const int splits = splits_of(type, z, rows, V, kPartVec * kThreads);
   unsigned long long* words = static_cast<unsigned long long*>(workspace);
@@ -1688,9 +1704,9 @@ cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, fl
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     const T* p = static_cast<const T*>(z.p);
-    const cudaError_t e = launch(kd_parts_kernel<T>, parts, stream, p, z.ld, rows, V, t, kLog2e * inv_t, words);
+    const cudaError_t e = launch(kd_parts_kernel<T>, parts, stream, p, z.ld, rows, V, t, (float)(kLog2ed / temp), words);
     if (e != cudaSuccess) return e;
-    return launch(kd_loss_kernel<T>, last, stream, p, z.ld, splits, V, t, kLog2e * inv_t, words, loss,
+    return launch(kd_loss_kernel<T>, last, stream, p, z.ld, splits, V, t, (float)(kLog2ed / temp), words, loss,
                   reinterpret_cast<KdRow*>(stats));
   });
 }
@@ -1699,7 +1715,7 @@ size_t kd_topk_grad_workspace(int64_t rows, int k) {
   carve_kd(rows, k, nullptr, bytes);
   return bytes;
 }
-cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight,
+cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
                          float* loss, void* out, int64_t out_ld, void* workspace, cudaStream_t stream) {
   size_t bytes;
   const KdRows r = carve_kd(rows, t.k, workspace, bytes);
@@ -1715,25 +1731,25 @@ cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, fl
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     const T* src = static_cast<const T*>(z.p);
-    const cudaError_t e = launch(kd_prepare_kernel<T>, prepare, stream, src, z.ld, V, t, kLog2e * inv_t, inv_t, weight, r);
+    const cudaError_t e = launch(kd_prepare_kernel<T>, prepare, stream, src, z.ld, V, t, (float)(kLog2ed / temp), 1.f / temp, weight, r);
     if (e != cudaSuccess) return e;
-    return launch(kd_grad_kernel<T>, grad, stream, src, z.ld, V, p.keep, t.k, kLog2e * inv_t, loss, static_cast<T*>(out),
+    return launch(kd_grad_kernel<T>, grad, stream, src, z.ld, V, p.keep, t.k, (float)(kLog2ed / temp), loss, static_cast<T*>(out),
                   out_ld, r);
   });
 }
-cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight,
+cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
                         const float* stats, void* out, int64_t out_ld, cudaStream_t stream) {
   Shape s;
   s.blocks = rows;
   s.units = splits_of(type, z, rows, V, kKdVec * kThreads);
   return by_type(type, [&](auto x) {
     using T = decltype(x);
-    return launch(kd_bwd_kernel<T>, s, stream, static_cast<const T*>(z.p), z.ld, rows, V, t, kLog2e * inv_t, inv_t, weight,
+    return launch(kd_bwd_kernel<T>, s, stream, static_cast<const T*>(z.p), z.ld, rows, V, t, (float)(kLog2ed / temp), 1.f / temp, weight,
                   reinterpret_cast<const KdRow*>(stats), static_cast<T*>(out), out_ld);
   });
 }
 
-cudaError_t accept_kl(Type type, Logits draft, Logits target, int64_t rows, int V, float inv_t, float* alpha, float* kl,
+cudaError_t accept_kl(Type type, Logits draft, Logits target, int64_t rows, int V, float temp, float* alpha, float* kl,
                       float* stats, cudaStream_t stream) {
   const Plan p = plan_of(type, rows, V, 2);
   Shape s;
@@ -1744,10 +1760,10 @@ cudaError_t accept_kl(Type type, Logits draft, Logits target, int64_t rows, int 
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     return launch(accept_kernel<T>, s, stream, static_cast<const T*>(draft.p), draft.ld, static_cast<const T*>(target.p),
-                  target.ld, V, p.keep, kLog2e * inv_t, alpha, kl, reinterpret_cast<AcceptRow*>(stats));
+                  target.ld, V, p.keep, (float)(kLog2ed / temp), temp, alpha, kl, reinterpret_cast<AcceptRow*>(stats));
   });
 }
-cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, int V, float inv_t, const float* stats,
+cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, int V, float temp, const float* stats,
                           const float* g_alpha, const float* g_kl, void* out, int64_t out_ld, cudaStream_t stream) {
   Shape s;
   s.blocks = rows;
@@ -1755,7 +1771,7 @@ cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, 
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     return launch(accept_bwd_kernel<T>, s, stream, static_cast<const T*>(draft.p), draft.ld,
-                  static_cast<const T*>(target.p), target.ld, rows, V, kLog2e * inv_t, inv_t,
+                  static_cast<const T*>(target.p), target.ld, rows, V, (float)(kLog2ed / temp), temp,
                   reinterpret_cast<const AcceptRow*>(stats), g_alpha, g_kl, static_cast<T*>(out), out_ld);
   });
 }

@@ -45,7 +45,7 @@ bool check_ids(const torch::Tensor& t, const torch::Tensor& like, const char* na
 }
 float check_temp(double t) {
   TORCH_CHECK(t >= 1e-6 && t <= 1e6, "temperature must be in [1e-6, 1e6], got ", t);
-  return (float)(1.0 / t);
+  return (float)t;
 }
 void launched(cudaError_t e, const char* what) {
   TORCH_CHECK(e == cudaSuccess, what, " launch failed: ", cudaGetErrorString(e));
@@ -65,11 +65,11 @@ void teacher_topk(torch::Tensor logits, double temp, torch::Tensor ids, torch::T
   const int64_t n = logits.size(0), k = ids.size(1);
   check_vec(ids, logits, n * k, torch::kInt32, "ids");
   check_vec(lp, logits, n * k, torch::kFloat, "lp");
-  const float inv_t = check_temp(temp);
+  const float t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(logits.device());
   const torch::Tensor ws = bytes_like(logits, v::teacher_topk_workspace(type_of(logits), rows_of(logits), n, logits.size(1), k));
-  launched(v::teacher_topk(type_of(logits), rows_of(logits), n, logits.size(1), k, inv_t, ids.data_ptr<int32_t>(),
+  launched(v::teacher_topk(type_of(logits), rows_of(logits), n, logits.size(1), k, t, ids.data_ptr<int32_t>(),
                            lp.data_ptr<float>(), ws.data_ptr(), at::cuda::getCurrentCUDAStream()),
            "teacher_topk");
 }
@@ -88,11 +88,11 @@ void kd_topk_loss(torch::Tensor logits, torch::Tensor t_ids, torch::Tensor t_lp,
   const int64_t n = logits.size(0);
   check_vec(loss, logits, n, torch::kFloat, "loss");
   if (stats) check_vec(*stats, logits, n * v::kKdStats, torch::kFloat, "stats");
-  const float inv_t = check_temp(temp);
+  const float t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(logits.device());
   const torch::Tensor ws = bytes_like(logits, v::kd_topk_loss_workspace(type_of(logits), rows_of(logits), n, logits.size(1)));
-  launched(v::kd_topk_loss(type_of(logits), rows_of(logits), n, logits.size(1), teacher, inv_t, loss.data_ptr<float>(),
+  launched(v::kd_topk_loss(type_of(logits), rows_of(logits), n, logits.size(1), teacher, t, loss.data_ptr<float>(),
                            opt(stats), ws.data_ptr(), at::cuda::getCurrentCUDAStream()), "kd_topk_loss");
 }
 
@@ -104,11 +104,11 @@ void kd_topk_grad(torch::Tensor logits, torch::Tensor t_ids, torch::Tensor t_lp,
   check_vec(loss, logits, n, torch::kFloat, "loss");
   check_vec(weight, logits, n, torch::kFloat, "weight");
   check_out(out, logits, "out");
-  const float inv_t = check_temp(temp);
+  const float t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(logits.device());
   const torch::Tensor ws = bytes_like(logits, v::kd_topk_grad_workspace(n, teacher.k));
-  launched(v::kd_topk_grad(type_of(logits), rows_of(logits), n, logits.size(1), teacher, inv_t, weight.data_ptr<float>(),
+  launched(v::kd_topk_grad(type_of(logits), rows_of(logits), n, logits.size(1), teacher, t, weight.data_ptr<float>(),
                            loss.data_ptr<float>(), out.data_ptr(), out.stride(0), ws.data_ptr(),
                            at::cuda::getCurrentCUDAStream()), "kd_topk_grad");
 }
@@ -120,10 +120,10 @@ void kd_topk_bwd(torch::Tensor logits, torch::Tensor t_ids, torch::Tensor t_lp, 
   check_vec(stats, logits, n * v::kKdStats, torch::kFloat, "stats");
   check_vec(weight, logits, n, torch::kFloat, "weight");
   check_out(out, logits, "out");
-  const float inv_t = check_temp(temp);
+  const float t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(logits.device());
-  launched(v::kd_topk_bwd(type_of(logits), rows_of(logits), n, logits.size(1), teacher, inv_t,
+  launched(v::kd_topk_bwd(type_of(logits), rows_of(logits), n, logits.size(1), teacher, t,
                           weight.data_ptr<float>(), stats.data_ptr<float>(), out.data_ptr(), out.stride(0),
                           at::cuda::getCurrentCUDAStream()), "kd_topk_bwd");
 }
@@ -142,10 +142,10 @@ void accept_kl(torch::Tensor draft, torch::Tensor target, double temp, torch::Te
   check_vec(alpha, draft, n, torch::kFloat, "alpha");
   check_vec(kl, draft, n, torch::kFloat, "kl");
   if (stats) check_vec(*stats, draft, n * v::kAcceptStats, torch::kFloat, "stats");
-  const float inv_t = check_temp(temp);
+  const float t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(draft.device());
-  launched(v::accept_kl(type_of(draft), rows_of(draft), rows_of(target), n, draft.size(1), inv_t,
+  launched(v::accept_kl(type_of(draft), rows_of(draft), rows_of(target), n, draft.size(1), t,
                         alpha.data_ptr<float>(), kl.data_ptr<float>(), opt(stats), at::cuda::getCurrentCUDAStream()),
            "accept_kl");
 }
@@ -158,10 +158,10 @@ void accept_kl_bwd(torch::Tensor draft, torch::Tensor target, double temp, torch
   check_vec(g_alpha, draft, n, torch::kFloat, "g_alpha");
   check_vec(g_kl, draft, n, torch::kFloat, "g_kl");
   check_out(out, draft, "out");
-  const float inv_t = check_temp(temp);
+  const float t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(draft.device());
-  launched(v::accept_kl_bwd(type_of(draft), rows_of(draft), rows_of(target), n, draft.size(1), inv_t,
+  launched(v::accept_kl_bwd(type_of(draft), rows_of(draft), rows_of(target), n, draft.size(1), t,
                             stats.data_ptr<float>(), g_alpha.data_ptr<float>(), g_kl.data_ptr<float>(), out.data_ptr(),
                             out.stride(0), at::cuda::getCurrentCUDAStream()), "accept_kl_bwd");
 }
@@ -217,6 +217,8 @@ void spec_verify(torch::Tensor logits, torch::Tensor drafts, torch::Tensor temps
 }  // namespace
 
 void register_vocab(pybind11::module& m) {
+  m.attr("kd_stats") = v::kKdStats;
+  m.attr("accept_stats") = v::kAcceptStats;
   m.def("teacher_topk", &teacher_topk);
   m.def("kd_topk_loss", &kd_topk_loss);
   m.def("kd_topk_grad", &kd_topk_grad);

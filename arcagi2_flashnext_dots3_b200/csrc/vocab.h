@@ -12,7 +12,7 @@ enum Type { F32 = 0, F16 = 1, BF16 = 2 };
 constexpr int kMaxK = 128;       // teacher tokens per row, drafts per sequence
 constexpr int kMaxV = 1 << 20;
 constexpr int kKdStats = 4;      // floats of per-row state between kd_topk and kd_topk_bwd
-constexpr int kAcceptStats = 5;  // floats of per-row state between accept_kl and accept_kl_bwd
+constexpr int kAcceptStats = 9;  // floats of per-row state between accept_kl and accept_kl_bwd
 
 struct Logits {
   const void* p;
@@ -28,23 +28,23 @@ struct Teacher {                 // [rows, k] ids (int32 or int64) and fp32 log-
 
 // A workspace has the bytes that its ..._workspace() says.
 size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V, int k);
-cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float inv_t, int32_t* ids, float* lp,
+cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float temp, int32_t* ids, float* lp,
                          void* workspace, cudaStream_t stream);
 
 // stats may be null
 size_t kd_topk_loss_workspace(Type type, Logits z, int64_t rows, int V);
-cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, float* loss, float* stats,
+cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, float* loss, float* stats,
                          void* workspace, cudaStream_t stream);
 // loss, and out = d sum(weight loss) / d logits; out may be the logits
 size_t kd_topk_grad_workspace(int64_t rows, int k);
-cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight,
+cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
                          float* loss, void* out, int64_t out_ld, void* workspace, cudaStream_t stream);
-cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float inv_t, const float* weight,
+cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
                         const float* stats, void* out, int64_t out_ld, cudaStream_t stream);
 
-cudaError_t accept_kl(Type type, Logits draft, Logits target, int64_t rows, int V, float inv_t, float* alpha, float* kl,
+cudaError_t accept_kl(Type type, Logits draft, Logits target, int64_t rows, int V, float temp, float* alpha, float* kl,
                       float* stats, cudaStream_t stream);
-cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, int V, float inv_t, const float* stats,
+cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, int V, float temp, const float* stats,
                           const float* g_alpha, const float* g_kl, void* out, int64_t out_ld, cudaStream_t stream);
 
 struct Verify {

@@ -113,21 +113,24 @@ def _kd_cpu(logits, t_ids, t_lp, t, weight=None):
     return loss, torch.where(nothing[:, None], 0.0, d).to(logits.dtype)
 
 
+def _kd_loss(logits, t_ids, t_lp, t, stats):
+    if not logits.is_cuda:
+        return _kd_cpu(logits, t_ids, t_lp, t)
+    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+    native.C().kd_topk_loss(logits, t_ids, t_lp, t, loss, stats)
+    return loss
+
+
 class _KDTopK(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, t_ids, t_lp, t):
         ctx.t = t
         if not logits.is_cuda:
             ctx.save_for_backward(logits, t_ids, t_lp)
-            return _kd_cpu(logits, t_ids, t_lp, t)
-        n = logits.shape[0]
-        loss = torch.empty(n, dtype=torch.float32, device=logits.device)
-        stats = None
-        if ctx.needs_input_grad[0]:
-            stats = torch.empty(n, 4, dtype=torch.float32, device=logits.device)
-            ctx.save_for_backward(logits, t_ids, t_lp, stats)
-        native.C().kd_topk_loss(logits, t_ids, t_lp, t, loss, stats)
-        return loss
+            return _kd_loss(logits, t_ids, t_lp, t, None)
+        stats = torch.empty(logits.shape[0], native.C().kd_stats, dtype=torch.float32, device=logits.device)
+        ctx.save_for_backward(logits, t_ids, t_lp, stats)
+        return _kd_loss(logits, t_ids, t_lp, t, stats)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -147,7 +150,10 @@ def kd_topk(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, tempe
     tail; a repeated id counts once, at its first place. Both tail masses have a floor of 1e-8."""
     logits = _rows(logits, "logits")
     t_ids, t_lp = _teacher(logits, t_ids, t_lp)
-    return _KDTopK.apply(logits, t_ids, t_lp, _temperature(temperature))
+    t = _temperature(temperature)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _KDTopK.apply(logits, t_ids, t_lp, t)
+    return _kd_loss(logits, t_ids, t_lp, t, None)
 
 
 def kd_topk_grad(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, weight: torch.Tensor,
@@ -186,9 +192,18 @@ def _accept_cpu(draft, target, t, g_alpha=None, g_kl=None):
         kl = torch.where(p > 0, p * (lp - lq), 0.0)
         kl = torch.where(torch.isnan(p), p, kl).sum(-1)
         return torch.where(nothing, 0.0, torch.minimum(q, p).sum(-1)), torch.where(nothing, 0.0, kl)
-    h = (lq <= lp).float()
+    h = (lq < lp).float() + 0.5 * (lq == lp).float()
     d = (g_alpha / t)[:, None] * q * (h - (q * h).sum(-1, keepdim=True)) + (g_kl / t)[:, None] * (q - p)
     return torch.where(nothing[:, None], 0.0, d).to(draft.dtype)
+
+
+def _accept(draft, target, t, stats):
+    if not draft.is_cuda:
+        return _accept_cpu(draft, target, t)
+    alpha = torch.empty(draft.shape[0], dtype=torch.float32, device=draft.device)
+    kl = torch.empty_like(alpha)
+    native.C().accept_kl(draft, target, t, alpha, kl, stats)
+    return alpha, kl
 
 
 class _AcceptKL(torch.autograd.Function):
@@ -197,16 +212,10 @@ class _AcceptKL(torch.autograd.Function):
         ctx.t = t
         if not draft.is_cuda:
             ctx.save_for_backward(draft, target)
-            return _accept_cpu(draft, target, t)
-        n = draft.shape[0]
-        alpha = torch.empty(n, dtype=torch.float32, device=draft.device)
-        kl = torch.empty_like(alpha)
-        stats = None
-        if ctx.needs_input_grad[0]:
-            stats = torch.empty(n, 5, dtype=torch.float32, device=draft.device)
-            ctx.save_for_backward(draft, target, stats)
-        native.C().accept_kl(draft, target, t, alpha, kl, stats)
-        return alpha, kl
+            return _accept(draft, target, t, None)
+        stats = torch.empty(draft.shape[0], native.C().accept_stats, dtype=torch.float32, device=draft.device)
+        ctx.save_for_backward(draft, target, stats)
+        return _accept(draft, target, t, stats)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -224,10 +233,13 @@ def accept_kl(draft: torch.Tensor, target: torch.Tensor, temperature: float = 1.
     """(alpha, kl) fp32 [rows] of draft logits against target logits of the same shape and type: alpha = sum_v
     min(q_v, p_v), the probability that speculative verification accepts a token drawn from q, and kl = KL(p || q),
     with q, p the softmaxes at `temperature`. Differentiable in the draft; the target is taken as given. Where q_v =
-    p_v the gradient of alpha is one of the subgradients. A row in which either side has no token left gives zeros."""
+    p_v the gradient of alpha is the mean of its two sides. A row in which either side has no token left gives zeros."""
     draft = _rows(draft, "draft logits")
     target = _rows(target.detach(), "target logits")
     if draft.shape != target.shape or draft.dtype != target.dtype or draft.device != target.device:
         raise ValueError(f"draft and target logits must agree in shape, type and device: {tuple(draft.shape)} "
                          f"{draft.dtype} {draft.device} and {tuple(target.shape)} {target.dtype} {target.device}")
-    return _AcceptKL.apply(draft, target, _temperature(temperature))
+    t = _temperature(temperature)
+    if draft.requires_grad and torch.is_grad_enabled():
+        return _AcceptKL.apply(draft, target, t)
+    return _accept(draft, target, t, None)
