@@ -1343,18 +1343,20 @@ __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, in
 
 // ------------------------------------------------------------------------------------------- draft verification
 // Two launches. The first reduces every needed row of logits, cut over blocks, to softmax parts (T > 0) or to its best
-// token (T <= 0). The second, one cluster per sequence and started early by programmatic launch, joins the parts, finds
-// the first rejected draft and draws from that position alone: the race costs a hash per token and is run for one row
+// token (T <= 0). The second, several blocks per sequence and started early by programmatic launch, joins the parts,
+// finds the first rejected draft and draws from that position alone: the race costs a hash per token and is run for one row
 // of the k + 1. A draw needs -log(u) / r below the best so far; -log(u) >= 1 - u, which is the hash's integer, so the
 // logarithm and the division are taken for the few tokens that can win.
-constexpr int kDrawThreads = 512;
+constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
+constexpr int kDrawVec = 2;          // vectors that a thread requests at once
 
-__device__ __forceinline__ uint32_t hash23(uint64_t base, uint64_t i) {   // the sampler's 23 random bits at index i
-  uint64_t z = base + i * 0x8CB92BA72F3D8DD7ull;
+constexpr uint64_t kIndexStep = 0x8CB92BA72F3D8DD7ull;
+// The sampler's 23 random bits of counter base + index kIndexStep.
+__device__ __forceinline__ uint32_t random23(uint64_t z) {
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-  return (uint32_t)(z >> 41);     // the last step, z ^ (z >> 31), leaves bits 33 and up as they are
+  return (uint32_t)(z >> 32) >> 9;     // the last step, z ^ (z >> 31), leaves bits 33 and up as they are
 }
 __device__ __forceinline__ float unit(uint32_t h) { return ((float)h + 0.5f) * (1.0f / 8388608.0f); }
 
@@ -1362,7 +1364,14 @@ __device__ __forceinline__ int drafts_of(const Verify& a, int64_t b) {
   return a.n_draft ? min(max(a.n_draft[b], 0), a.k) : a.k;
 }
 
-// parts [batch][2 k + 1 rows: k + 1 of the target, k of the draft][splits], 8 bytes: Soft, or a rank_key
+// Workspace: best draw and arrivals of each sequence, then parts [batch][2 k + 1 rows: k + 1 of the target, k of the
+// draft][splits], 8 bytes each: Soft, or a rank_key.
+__device__ __forceinline__ unsigned long long* verify_best(const Verify& a) {
+  return static_cast<unsigned long long*>(a.workspace);
+}
+__device__ __forceinline__ unsigned long long* verify_count(const Verify& a) { return verify_best(a) + a.batch; }
+__device__ __forceinline__ unsigned long long* verify_parts(const Verify& a) { return verify_best(a) + 2 * a.batch; }
+
 template <typename T, int kUnroll>
 __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int splits) {
   constexpr int N = Vec<T>::N;
@@ -1372,6 +1381,10 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
   const int j = (blockIdx.x / splits) % rows;
   const int64_t b = blockIdx.x / splits / rows;
   pdl_launch_dependents();
+  if (j == 0 && split == 0 && threadIdx.x == 0) {
+    verify_best(a)[b] = kNone;
+    verify_count(a)[b] = 0;
+  }
   const int n = drafts_of(a, b);
   const float temp = a.temps[b];
   const bool draft = j > a.k, greedy = !(temp > 0.f);
@@ -1409,18 +1422,19 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
     const Soft t = join_parts(kWarps, kl, [&](int i) { return warp_part[i]; });
     res = as_u64(t.c, t.sum);
   }
-  if (threadIdx.x == 0) static_cast<unsigned long long*>(a.workspace)[blockIdx.x] = res;
+  if (threadIdx.x == 0) verify_parts(a)[blockIdx.x] = res;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify a, int splits, int per) {
+__global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, int splits, int blocks, int per) {
   constexpr int N = Vec<T>::N;
   __shared__ Soft s_p[kMaxK + 1], s_q[kMaxK];
   __shared__ unsigned long long s_best[kMaxK + 1];
   __shared__ int s_ok[kMaxK + 1];
-  __shared__ unsigned long long warp_best[kDrawWarps], part[2][kMaxCluster];
-  const uint32_t rank = cluster_rank(), size = cluster_size();
-  const int64_t b = blockIdx.x / size;
+  __shared__ unsigned long long warp_best[kDrawWarps];
+  __shared__ bool s_again;
+  const int rank = blockIdx.x % blocks;
+  const int64_t b = blockIdx.x / blocks;
   const int tid = threadIdx.x, lane = tid & 31;
   const int rows = a.draft_logits ? 2 * a.k + 1 : a.k + 1;
   pdl_wait();
@@ -1429,7 +1443,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify a, int
   const bool greedy = !(temp > 0.f);
   const float kl = greedy ? 1.f : kLog2e / temp;
   const uint64_t seed = (uint64_t)a.seeds[b] * 0x9E3779B97F4A7C15ull + 1ull, step = (uint64_t)a.steps[b];
-  const unsigned long long* parts = static_cast<const unsigned long long*>(a.workspace) + b * rows * splits;
+  const unsigned long long* parts = verify_parts(a) + b * rows * splits;
   for (int j = tid >> 5; j <= n; j += kDrawWarps) {     // one warp per position
     const int64_t id = j < n ? (a.wide ? static_cast<const int64_t*>(a.drafts)[b * a.k + j]
                                        : (int64_t) static_cast<const int32_t*>(a.drafts)[b * a.k + j])
@@ -1468,7 +1482,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify a, int
           const float zq = Vec<T>::one(static_cast<const T*>(a.draft_logits)[b * a.draft_b + j * a.draft_j + id]);
           qd = q.sum > 0.f ? ex2(fmaf(zq, kl, -q.c)) / q.sum : 0.f;
         }
-        ok = unit(hash23(seed + (step + j) * 0xD1B54A32D192ED03ull, ~0ull)) * qd < pd;
+        ok = unit(random23(seed + (step + j) * 0xD1B54A32D192ED03ull - kIndexStep)) * qd < pd;   // index -1
       }
       s_ok[j] = ok;
     }
@@ -1483,70 +1497,81 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify a, int
     }
     return;
   }
-  cluster_started();
   const T* row = static_cast<const T*>(a.logits) + b * a.logits_b + acc * a.logits_j;
   const T* qrow = a.draft_logits && acc < n ? static_cast<const T*>(a.draft_logits) + b * a.draft_b + acc * a.draft_j : nullptr;
   const int64_t id = acc >= n ? -1 : a.wide ? static_cast<const int64_t*>(a.drafts)[b * a.k + acc]
                                             : (int64_t) static_cast<const int32_t*>(a.drafts)[b * a.k + acc];
-  const Slice<T> s(row, a.V, per, rank);
   const Soft p = s_p[acc];
   const float ip = 1.f / p.sum, cq = qrow ? s_q[acc].c : 0.f, iq = qrow && s_q[acc].sum > 0.f ? 1.f / s_q[acc].sum : 0.f;
   const bool same = ((reinterpret_cast<uintptr_t>(qrow) ^ reinterpret_cast<uintptr_t>(row)) & 15) == 0;
   const uint64_t base = seed + (step + acc) * 0xD1B54A32D192ED03ull;
-  unsigned long long best = kNone;
-  cluster_peers_run();
-  for (int whole = acc == n; whole < 2 && best == kNone; ++whole) {   // second round: an empty residual leaves p itself
-    float bound = INFINITY;                                           // the best of this warp
-    for (int v0 = tid - lane; v0 < s.count; v0 += kDrawThreads) {     // the same trip count for a whole warp
-      const int v = v0 + lane, i0 = s.start(v);
-      if (v < s.count) {
-        float f[N], g[N];
-        if (s.full(i0)) {
-          Vec<T>::unpack(*reinterpret_cast<const uint4*>(row + i0), f);
-        } else {
+  // The block that completes a sequence finds an empty residual, and then draws from p itself, all of the row alone.
+  for (int whole = acc == n, mine = 1;; whole = 1, mine = 0) {
+    const Slice<T> s(row, a.V, mine ? per : a.V, mine ? rank : 0);
+    unsigned long long best = kNone;
+    float bound = INFINITY;                                           // of this warp: its best time, rounded up
+    for (int v0 = tid; v0 - lane < s.count; v0 += kDrawVec * kDrawThreads) {   // the same trip count for a whole warp
+      uint4 xp[kDrawVec], xq[kDrawVec];
 #pragma unroll
-          for (int k = 0; k < N; ++k) f[k] = i0 + k >= 0 && i0 + k < a.V ? Vec<T>::one(row[i0 + k]) : -INFINITY;
-        }
-        if (qrow && !whole) {
-          if (same && s.full(i0)) {
-            Vec<T>::unpack(*reinterpret_cast<const uint4*>(qrow + i0), g);
-          } else {
-#pragma unroll
-            for (int k = 0; k < N; ++k) g[k] = i0 + k >= 0 && i0 + k < a.V ? Vec<T>::one(qrow[i0 + k]) : -INFINITY;
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          float r = ex2(fmaf(f[k], kl, -p.c)) * ip;
-          if (!whole) {
-            if (qrow) r -= ex2(fmaf(g[k], kl, -cq)) * iq;
-            else if (i0 + k == id) r = 0.f;
-          }
-          const uint32_t h = hash23(base, (uint64_t)(uint32_t)(i0 + k));
-          const float miss = (float)(8388607u - h) + 0.5f;            // (1 - u) 2^23
-          if (r > 0.f && miss * (0.999999f / 8388608.0f) <= bound * r) {
-            const float e = -logf(unit(h)) / r;
-            best = min(best, (unsigned long long)__float_as_uint(e) << 32 | (uint32_t)(i0 + k));
-            bound = fminf(bound, e);
-          }
+      for (int i = 0; i < kDrawVec; ++i) {
+        const int v = v0 + i * kDrawThreads, i0 = s.start(v);
+        xp[i] = xq[i] = make_uint4(Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad);
+        if (v < s.count) {
+          xp[i] = s.full(i0) ? __ldcs(reinterpret_cast<const uint4*>(row + i0)) : ragged_vec(s, row, i0);
+          if (qrow && !whole)
+            xq[i] = same && s.full(i0) ? __ldcs(reinterpret_cast<const uint4*>(qrow + i0)) : ragged_vec(s, qrow, i0);
         }
       }
-      bound = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(bound)));
+#pragma unroll
+      for (int i = 0; i < kDrawVec; ++i) {
+        if (v0 - lane + i * kDrawThreads >= s.count) break;            // for the whole warp
+        const int i0 = s.start(v0 + i * kDrawThreads);
+        float f[N], g[N];
+        Vec<T>::unpack(xp[i], f);
+        Vec<T>::unpack(xq[i], g);
+        uint64_t counter = base + (uint64_t)(int64_t)i0 * kIndexStep;
+#pragma unroll
+        for (int k = 0; k < N; ++k, counter += kIndexStep) {
+          float r = ex2(fmaf(f[k], kl, -p.c)) * ip;
+          if (!whole) {
+            if (qrow) r = fmaf(ex2(fmaf(g[k], kl, -cq)), -iq, r);
+            else if (i0 + k == id) r = 0.f;
+          }
+          // u = (h + 1/2) 2^-23 and 1 - u, from the fraction bits h of 1 + h 2^-23; -log(u) > 1 - u
+          const uint32_t h = random23(counter);
+          const float miss = (2.f - __uint_as_float(0x3F800000u | h)) - 0x1p-24f;
+          if (miss <= bound * r) {                                    // false for r <= 0, and where r is NaN
+            const float e = -logf(unit(h)) / r;
+            best = min(best, (unsigned long long)__float_as_uint(e) << 32 | (uint32_t)(i0 + k));
+            bound = fminf(bound, e * 1.000001f);
+          }
+          if (k == 0 || k == N / 2)                                   // early, or a warp's first vector takes all logarithms
+            bound = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(bound)));
+        }
+        bound = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(bound)));
+      }
     }
     best = warp_reduce(best, MinKey());
     if (lane == 0) warp_best[tid >> 5] = best;
     __syncthreads();
-    if (tid < 32) {
-      best = warp_reduce(warp_best[tid & (kDrawWarps - 1)], MinKey());
-      if (tid < (int)size) st_peer(&part[whole][rank], tid, best);
+    if (tid == 0) {
+      for (int i = 1; i < kDrawWarps; ++i) best = min(best, warp_best[i]);
+      s_again = false;
+      bool last = !mine;
+      if (mine) {
+        atomicMin(verify_best(a) + b, best);
+        __threadfence();
+        last = atomicAdd(verify_count(a) + b, 1ull) == (unsigned long long)(blocks - 1);
+        if (last) best = atomicMin(verify_best(a) + b, kNone);
+      }
+      if (last) {
+        s_again = best == kNone && !whole;
+        a.accepted[b] = acc;
+        a.next[b] = best == kNone ? -1 : (int)(uint32_t)best;
+      }
     }
-    cluster_sync();
-    best = kNone;
-    for (uint32_t i = 0; i < size; ++i) best = min(best, part[whole][i]);
-  }
-  if (rank == 0 && tid == 0) {
-    a.accepted[b] = acc;
-    a.next[b] = best == kNone ? -1 : (int)(uint32_t)best;
+    __syncthreads();
+    if (!s_again) return;
   }
 }
 
@@ -1791,7 +1816,7 @@ VerifyPlan verify_plan(const Verify& a) {
 
 size_t spec_verify_workspace(const Verify& a) {
   const VerifyPlan p = verify_plan(a);
-  return (size_t)a.batch * p.rows * p.splits * 8;
+  return ((size_t)a.batch * p.rows * p.splits + 2 * a.batch) * 8;
 }
 
 cudaError_t spec_verify(const Verify& a, cudaStream_t stream) {
@@ -1803,14 +1828,14 @@ cudaError_t spec_verify(const Verify& a, cudaStream_t stream) {
     cudaError_t e = launch(p.unroll == 8 ? verify_parts_kernel<T, 8> : verify_parts_kernel<T, 2>, parts, stream, a,
                            p.splits);
     if (e != cudaSuccess) return e;
+    // four blocks per SM over all sequences, each of at least one vector per thread
     const int total = (a.V + Vec<T>::N - 1) / Vec<T>::N + 1;
-    int c = 1;
-    while (c < kMaxCluster && total > kDrawThreads * c && (c < 8 || a.batch * c < sm_count())) c *= 2;
+    const int64_t most = (total + kDrawThreads - 1) / kDrawThreads, want = (4 * sm_count() + a.batch - 1) / a.batch;
+    const int c = (int)std::min(most, want);
     draw.blocks = a.batch * c;
     draw.threads = kDrawThreads;
-    draw.cluster = c;
     draw.early = true;
-    return launch(verify_draw_kernel<T>, draw, stream, a, p.splits, (total + c - 1) / c);
+    return launch(verify_draw_kernel<T>, draw, stream, a, p.splits, c, (total + c - 1) / c);
   });
 }
 
