@@ -9,7 +9,7 @@ flashnext/training/draft_head/train.py); its code works in torch on whole [rows,
 * :func:`accept_kl` - sum min(q, p) and KL(p || q) of a draft distribution q against a target p, differentiable in
   the draft.
 
-Logits are [rows, vocab] in fp32, fp16 or bf16 (vocab up to 393216; rows may be strided). A logit at or below -1e30
+Logits are [rows, vocab] in fp32, fp16 or bf16 (vocab up to 2^20; rows may be strided). A logit at or below -1e30
 (-inf, the lowest fp32 / bf16 value) is masked and has probability 0; a row with nothing left gives loss 0, gradient
 0 and id -1. A NaN makes its row's results NaN. Results per row are fp32, gradients have the logits' type. Nothing
 here reads from the host, so every call can be captured in a CUDA graph.
@@ -22,13 +22,14 @@ from . import native
 
 MASKED = -1e30       # csrc/k_vocab.cu kMasked
 TAIL_FLOOR = 1e-8    # csrc/k_vocab.cu kTailFloor
-MAX_K = 128          # csrc/k_vocab.cu kMaxK
+MAX_K = 128          # csrc/vocab.h kMaxK
+DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"{name}: expected [rows, vocab], got {tuple(x.shape)}")
-    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if x.dtype not in DTYPES:
         raise ValueError(f"{name}: fp32, fp16 or bf16 logits, got {x.dtype}")
     return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
 

@@ -15,6 +15,7 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 from ..models import d3_reference as R
+from ..ops import distill
 from .lowbit import ExpertBank, grouped_experts
 from .student import _to
 
@@ -161,8 +162,11 @@ def sft_loss(model, ids: torch.Tensor, resp_start: int, chunk: int = 1024) -> to
 def kd_topk_loss(student_logits: torch.Tensor, t_ids: torch.Tensor, t_logprobs: torch.Tensor) -> torch.Tensor:
     """KL(teacher || student) over the teacher's top-k tokens plus one tail bin (the reference's 21-bin top-20
     KL, flashnext/training/kd/train_kd.py). student_logits [n, V]; t_ids, t_logprobs [n, k]."""
+    if student_logits.dim() == 2 and student_logits.dtype in distill.DTYPES and t_ids.shape[-1] <= distill.MAX_K and \
+            not t_logprobs.requires_grad:
+        return distill.kd_topk(student_logits, t_ids.long(), t_logprobs).mean()
     ls = torch.log_softmax(student_logits.float(), -1)
-    ps_top = ls.gather(1, t_ids.long())
+    ps_top = ls.gather(-1, t_ids.long())
     pt_top = t_logprobs.float().exp()
     tail_t = (1 - pt_top.sum(-1)).clamp_min(1e-8)
     tail_s = (1 - ps_top.exp().sum(-1)).clamp_min(1e-8)

@@ -17,7 +17,8 @@ instead holds step-1 entries for past positions.
 Objective per start position q: alpha_k = sum_v min(q_k(v), p_k(v)), the probability that draft k is accepted
 when drafts are sampled from q_k and verified against the target distribution p_k (the main model's next-token
 distribution at position q + k, renormalized over the hot vocabulary). E = sum_k prod_{j <= k} alpha_j is the
-expected number of accepted drafts. loss = -mean(E) + kl_weight * mean_k KL(p_k || q_k).
+expected number of accepted drafts. loss = -mean(E) + kl_weight * mean_k KL(p_k || q_k). alpha_k and
+the KL of a step come from :func:`..ops.distill.accept_kl`.
 """
 from __future__ import annotations
 
@@ -26,6 +27,7 @@ import torch.nn as nn
 
 from ..models import fn_reference as R
 from ..models.fn_mtp import mtp_config
+from ..ops import distill
 from .student import FNStudent
 
 
@@ -114,12 +116,10 @@ def draft_objective(model: DraftHeadTrain, h_main: torch.Tensor, ids: torch.Tens
     kl = x.new_zeros(())
     for k in range(1, K + 1):
         x = model.step(x, ids[k:k + Q], k - 1)
-        lq = torch.log_softmax(model.logits(x), -1)
-        lp = torch.log_softmax(tl[k:k + Q], -1)
-        p = lp.exp()
-        prod = prod * torch.minimum(lq.exp(), p).sum(-1)
+        alpha, kl_k = distill.accept_kl(model.logits(x).float(), tl[k:k + Q])
+        prod = prod * alpha
         E = E + prod
-        kl = kl + (p * (lp - lq)).sum(-1).mean()
+        kl = kl + kl_k.mean()
     return -E.mean() + kl_weight * kl / K, E.mean().detach()
 
 

@@ -10,8 +10,10 @@ Record format (``*.npz``): ``ids`` int32 [L], ``plen`` int (prompt length), ``ge
 generated positions, ``top_ids`` int32 [n_gen, K] / ``top_lp`` fp32 [n_gen, K] teacher top-K per generated
 position in order (id -1 pads unused slots).
 
-The student's log-probabilities at the teacher's K tokens come from :class:`VocabTopK`, which keeps only the
-hidden rows and recomputes each row chunk's [rows, vocab] projection in backward.
+The loss runs through :class:`VocabKD`: each row chunk's [rows, vocab] projection is overwritten by its own gradient
+(:func:`..ops.distill.kd_topk_grad`) and projected back at once, so backward needs no second projection and no
+vocabulary-sized activation outlives its chunk. (:class:`VocabTopK` + :func:`kl21` are the same loss with the projection
+recomputed in backward.) :func:`dump_records` writes the records from an engine model.
 
     python -m arcagi2_flashnext_dots3_b200.training.kd --data DIR --build BUILD --out OUT [--steps N]
 """
@@ -27,6 +29,8 @@ from pathlib import Path
 import numpy as np
 import torch
 import torch.distributed as dist
+
+from ..ops import distill
 
 TOOL_OPEN, TOOL_CLOSE = 248058, 248059   # FN chat template's tool-call delimiters
 
@@ -79,6 +83,48 @@ def kl21(student_lp_k: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor):
     return top + tail_t * (tail_t.log() - tail_s.log())
 
 
+class VocabKD(torch.autograd.Function):
+    """Distillation loss of hidden rows h [n, H] through the LM head W [V, H]: (sum of weight * kl, kl [n], whether the
+    student's best of the teacher's K tokens is the teacher's first [n]). ``weight`` fp32 [n]; only the sum is
+    differentiable. The weights are known, so forward takes each chunk's logits to their gradient in place, and backward
+    only scales by the incoming gradient of the sum."""
+
+    @staticmethod
+    def forward(ctx, h, W, t_ids, t_lp, weight, rows: int):
+        Wf = W.float()
+        n = h.shape[0]
+        kl = torch.empty(n, dtype=torch.float32, device=h.device)
+        first = torch.empty(n, dtype=torch.bool, device=h.device)
+        dh = torch.empty(h.shape, dtype=torch.float32, device=h.device) if ctx.needs_input_grad[0] else None
+        dW = torch.zeros_like(Wf) if ctx.needs_input_grad[1] else None
+        for s in range(0, n, rows):
+            e = min(n, s + rows)
+            hs = h[s:e].float()
+            z = hs @ Wf.t()
+            ids = t_ids[s:e]
+            at_k = z.gather(1, ids.long().clamp(0, W.shape[0] - 1)).masked_fill(ids < 0, float("-inf"))
+            first[s:e] = at_k.argmax(1) == 0
+            if dh is None and dW is None:
+                kl[s:e] = distill.kd_topk(z, ids, t_lp[s:e])
+                continue
+            kl[s:e], d = distill.kd_topk_grad(z, ids, t_lp[s:e], weight[s:e], out=z)
+            if dh is not None:
+                torch.mm(d, Wf, out=dh[s:e])
+            if dW is not None:
+                dW.addmm_(d.t(), hs)
+        ctx.save_for_backward(dh, dW)
+        ctx.types = h.dtype, W.dtype
+        ctx.mark_non_differentiable(kl, first)
+        return (kl * weight).sum(), kl, first
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _kl, _first):
+        dh, dW = ctx.saved_tensors
+        return ((dh * g).to(ctx.types[0]) if dh is not None else None,
+                (dW * g).to(ctx.types[1]) if dW is not None else None, None, None, None, None)
+
+
 def load_record(path, max_len: int = 0):
     """(ids, positions scored, teacher ids, teacher log-probs) of one record; position p is scored from the
     hidden state at p - 1, so the first position and prompt positions are never scored."""
@@ -122,12 +168,15 @@ def seq_kd(model, path, chunk: int = 1024, grad: bool = True, w_tool: float = 1.
         at = torch.as_tensor(pos, device=dev)
         tid_t = torch.as_tensor(tid, dtype=torch.long, device=dev)
         rows = h.index_select(0, at - 1)
-        lp_k = VocabTopK.apply(rows, model.lm_head, tid_t.clamp_min(0), max(1, chunk))
-        kl = kl21(lp_k, tid_t, torch.as_tensor(tlp, device=dev))
         w = torch.as_tensor(tool_weights(ids, pos, w_tool), device=dev)
-        loss = (kl * w).sum()
-    agree = float((lp_k.detach().argmax(1) == 0).float().sum())   # student's best of the K is the teacher's top-1
-    return loss, {"kl": float(kl.detach().sum()), "n": len(pos), "agree": agree}
+        tlp_t = torch.as_tensor(tlp, device=dev)
+        if tid_t.shape[1] <= distill.MAX_K:
+            loss, kl, first = VocabKD.apply(rows, model.lm_head, tid_t, tlp_t, w, max(1, chunk))
+        else:                                       # records of more tokens than the kernels list
+            lp_k = VocabTopK.apply(rows, model.lm_head, tid_t.clamp_min(0), max(1, chunk))
+            kl = kl21(lp_k, tid_t, tlp_t)
+            loss, kl, first = (kl * w).sum(), kl.detach(), lp_k.detach().argmax(1) == 0
+    return loss, {"kl": float(kl.sum()), "n": len(pos), "agree": float(first.sum())}
 
 
 def write_kd_records(out_dir, seqs):
@@ -137,6 +186,49 @@ def write_kd_records(out_dir, seqs):
         np.savez(os.path.join(out_dir, f"kd-{i:05d}.npz"), ids=np.asarray(ids, np.int32), plen=np.int64(plen),
                  gen=np.asarray(gen, np.int64).reshape(-1, 2), top_ids=np.asarray(tid, np.int32),
                  top_lp=np.asarray(tlp, np.float32))
+
+
+@torch.no_grad()
+def dump_records(llm, seqs, out_dir, k: int = 20, chunk: int = 512, temperature: float = 1.0) -> int:
+    """Teacher records of an engine model (the reference's kd/dump.py): every sequence of ``seqs`` (token ids, prompt
+    length) is run through the engine step chunk by chunk, and the top-k tokens of its generated positions are kept
+    (:func:`..ops.distill.teacher_topk`). Returns the number of positions recorded."""
+    dev, m, recs, total = llm.device, llm.model, [], 0
+    if getattr(m, "vocab_sharded", False):
+        raise NotImplementedError("teacher records over a vocabulary-sharded LM head")
+    for ids, plen in seqs:
+        L = len(ids)
+        if not 1 <= plen <= L:
+            raise ValueError(f"prompt length {plen} of a sequence of {L} tokens")
+        if L > llm.ec.max_model_len:
+            raise ValueError(f"sequence of {L} tokens > max_model_len {llm.ec.max_model_len}")
+        if not llm.free_slots:
+            raise RuntimeError("no free sequence slot")
+        slot = llm.free_slots.pop()
+        try:
+            m.reset_slot(slot)
+            m.assign_blocks(slot, L, llm.alloc)
+            t_all = torch.tensor(ids, dtype=torch.int32)
+            tid, tlp = [], []
+            for p0 in range(0, L - 1, chunk):            # the hidden state of position p predicts token p + 1
+                n = min(chunk, L - 1 - p0)
+                x = m.step(t_all[p0:p0 + n].to(dev), torch.tensor([slot], dtype=torch.int32, device=dev),
+                           torch.tensor([p0], dtype=torch.int32, device=dev), n)
+                first = max(0, plen - 1 - p0)
+                if first < n:
+                    i, lp = distill.teacher_topk(m.logits(x[first:]), k, temperature)
+                    tid.append(i.cpu())
+                    tlp.append(lp.cpu())
+        finally:
+            llm.alloc.release(slot)
+            m.reset_slot(slot)
+            llm.free_slots.append(slot)
+        tid = torch.cat(tid) if tid else torch.empty(0, k, dtype=torch.int32)
+        tlp = torch.cat(tlp) if tlp else torch.empty(0, k)
+        recs.append((ids, plen, [[plen, L]], tid.numpy(), tlp.numpy()))
+        total += L - plen
+    write_kd_records(out_dir, recs)
+    return total
 
 
 def main(argv=None):
