@@ -10,6 +10,7 @@ Commands (each forwards its arguments to the module named):
   spec-bench     speculative decoding (launch.spec_bench)   d3-bench      D3 decode (launch.d3_bench)
   kbench         kernel microbenchmarks (launch.kbench)     ref-kernels   reference kernels vs ours
   compare        build comparison (evaluation.compare)      paired        paired bootstrap (evaluation.paired)
+  distill-demo   teacher records, distillation, draft head and sampled drafting on a small model (launch.distill_demo)
 """
 from __future__ import annotations
 
@@ -25,6 +26,7 @@ COMMANDS = {
     "package": "launch.package", "serve-bench": "launch.serve_bench", "spec-bench": "launch.spec_bench",
     "d3-bench": "launch.d3_bench", "kbench": "launch.kbench", "ref-kernels": "launch.ref_kernels",
     "compare": "evaluation.compare", "paired": "evaluation.paired",
+    "distill-demo": "launch.distill_demo",
 }
 
 

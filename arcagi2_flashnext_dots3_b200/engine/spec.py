@@ -21,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from ..ops import fn_ops as ops
+from ..ops import sampling
 from .block_manager import BlockAllocator
 from .llm import greedy_ids
 
@@ -125,12 +126,17 @@ class SpecGraph:
     row, count accepted drafts on the device (leading matches of drafts and verify argmaxes), commit the recurrent
     states with those counts and, with an MTP head, run the head over the accepted rows and chain its next k
     drafts, all without a host round trip. The accepted rows' next tokens are exactly the verify argmaxes
-    y[0..a], which is what the head reads. Padding rows use the engine's scratch slot."""
+    y[0..a], which is what the head reads. With ``sampled``, rows of temperature > 0 verify by rejection sampling
+    (ops.sampling.speculative_verify) and y holds the accepted drafts and the token drawn after them. Padding rows
+    use the engine's scratch slot (and are greedy)."""
 
-    def __init__(self, llm, head, batch: int, k: int):
+    def __init__(self, llm, head, batch: int, k: int, sampled: bool = False):
         dev = llm.device
-        self.llm, self.head, self.B, self.k = llm, head, batch, k
+        self.llm, self.head, self.B, self.k, self.sampled = llm, head, batch, k, sampled
         k1 = k + 1
+        self.temps = torch.zeros(batch, device=dev)
+        self.seeds = torch.zeros(batch, dtype=torch.int64, device=dev)
+        self.steps = torch.zeros(batch, dtype=torch.int64, device=dev)
         self.ids = torch.zeros(batch, k1, dtype=torch.int32, device=dev)
         self.slots = torch.full((batch,), llm.scratch, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(batch, dtype=torch.int32, device=dev)
@@ -142,9 +148,16 @@ class SpecGraph:
     def _body(self):
         m, B, k, k1 = self.llm.model, self.B, self.k, self.k + 1
         x = m.step(self.ids.view(-1), self.slots, self.pos, k1, verify=True)
-        y = greedy_ids(m, x).view(B, k1)
-        match = (self.ids[:, 1:] == y[:, :k]).to(torch.int32)
-        acc = torch.cumprod(match, 1).sum(1).to(torch.int32)
+        if self.sampled:
+            drafts = self.ids[:, 1:].contiguous()
+            acc, nxt = sampling.speculative_verify(m.logits(x).view(B, k1, -1), drafts, self.temps, self.seeds, self.steps)
+            at = torch.arange(k1, device=x.device)[None]
+            y = torch.where(at < acc[:, None], torch.cat([drafts, nxt[:, None]], 1),
+                            torch.where(at == acc[:, None], nxt[:, None], 0)).clamp_min(0)
+        else:
+            y = greedy_ids(m, x).view(B, k1)
+            match = (self.ids[:, 1:] == y[:, :k]).to(torch.int32)
+            acc = torch.cumprod(match, 1).sum(1).to(torch.int32)
         m.commit(acc + 1)
         self.y.copy_(y)
         self.acc.copy_(acc)
@@ -201,19 +214,19 @@ class SpecDecoder:
             llm._keep_prefill_rows = False
         return seq
 
-    def _graph_step(self, seqs, drafts):
+    def _graph_step(self, seqs, drafts, sampled: bool = False):
         """Verify + commit (+ MTP chain) as one graph replay; returns (y rows, accepted counts) as host lists."""
         llm, k = self.llm, self.k
         k1 = k + 1
         n = len(seqs)
         bucket = next((b for b in llm.ec.graph_batch_sizes if b >= n), n)
-        g = self.graphs.get(bucket)
+        g = self.graphs.get((bucket, sampled))
         head = self.drafter.head if isinstance(self.drafter, MTPDrafter) else None
         if g is None:
             if head is not None:
                 head.assign_blocks(llm.scratch, 2 * k1 + 8, self.drafter.alloc)
             llm.model.assign_blocks(llm.scratch, k1 + 1, llm.alloc)
-            g = self.graphs[bucket] = SpecGraph(llm, head, bucket, k)
+            g = self.graphs[bucket, sampled] = SpecGraph(llm, head, bucket, k, sampled)
             g.capture()
         for s in seqs:
             llm.model.assign_blocks(s.slot, s.pos + k1 + 1, llm.alloc)
@@ -224,6 +237,10 @@ class SpecDecoder:
         g.ids.copy_(torch.tensor(ids, dtype=torch.int32))
         g.slots.copy_(torch.tensor([s.slot for s in seqs] + [llm.scratch] * pad, dtype=torch.int32))
         g.pos.copy_(torch.tensor([s.pos for s in seqs] + [0] * pad, dtype=torch.int32))
+        if sampled:
+            g.temps.copy_(torch.tensor([s.sp.temperature for s in seqs] + [0.0] * pad, dtype=torch.float32))
+            g.seeds.copy_(torch.tensor([s.sp.seed for s in seqs] + [0] * pad, dtype=torch.int64))
+            g.steps.copy_(torch.tensor([len(s.out) for s in seqs] + [0] * pad, dtype=torch.int64))
         g.run()
         out = torch.cat([g.y, g.acc[:, None], g.nd], 1).cpu()
         y = out[:n, :k1].tolist()
@@ -244,8 +261,8 @@ class SpecDecoder:
             raise ValueError("speculative sampling supports full-vocabulary temperature sampling (no top-k / top-p)")
         dev = llm.device
         drafts = self.drafter.propose(llm, seqs, k)
-        if self.use_graph and not sampled:
-            y, accepted = self._graph_step(seqs, drafts)
+        if self.use_graph and not (sampled and getattr(llm.model, "vocab_sharded", False)):
+            y, accepted = self._graph_step(seqs, drafts, sampled)
             return self._advance(seqs, drafts, y, accepted)
         ids = [[s.out[-1]] + list(d) for s, d in zip(seqs, drafts)]
         for s in seqs:
@@ -270,10 +287,9 @@ class SpecDecoder:
         return res
 
     def _sample_verify(self, seqs, x, drafts):
-        """Rejection-sampling verification (ops.sampling.speculative_accept; the sharded form when the LM head is
-        split over a TP group). Emitted tokens follow the model's sampling distribution; greedy rows in the batch
-        verify by argmax as before."""
-        from ..ops import sampling
+        """Rejection-sampling verification (ops.sampling.speculative_verify on the GPU, speculative_accept on the CPU,
+        the sharded form when the LM head is split over a TP group). Emitted tokens follow the model's sampling
+        distribution; greedy rows in the batch verify by argmax as before."""
         m, k1 = self.llm.model, self.k + 1
         dr = torch.tensor([list(d) for d in drafts], dtype=torch.long).view(len(seqs), self.k)
         temps = [s.sp.temperature for s in seqs]
@@ -283,8 +299,13 @@ class SpecDecoder:
             from ..parallel.tp import sharded_speculative_accept
             lg = m._mm(x, m.W["lm_head"], f8=False).float().view(len(seqs), k1, -1)
             return sharded_speculative_accept(lg, m.W["vocab_range"][0], dr, temps, seeds, steps, m.tp.group)
-        lg = m.logits(x).float().view(len(seqs), k1, -1)
-        return sampling.speculative_accept(lg, dr, temps, seeds, steps)
+        lg = m.logits(x).view(len(seqs), k1, -1)
+        if lg.is_cuda:
+            t = [torch.tensor(v, dtype=ty).to(lg.device) for v, ty in
+                 ((temps, torch.float32), (seeds, torch.int64), (steps, torch.int64))]
+            acc, nxt = sampling.speculative_verify(lg, dr.to(lg.device), *t)
+            return acc.tolist(), nxt.clamp_min(0).tolist()
+        return sampling.speculative_accept(lg.float(), dr, temps, seeds, steps)
 
     def _advance(self, seqs, drafts, y, accepted) -> dict:
         llm, k = self.llm, self.k
