@@ -38,7 +38,6 @@
 //     probability alike, so that rounding cancels; one FMA and one ex2 per element.
 #include <algorithm>
 #include <cstdint>
-#include <cstdlib>
 #include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -55,8 +54,10 @@ constexpr int kBatch = 8;            // vectors that a thread holds at once
 constexpr int kMaxCluster = 16;
 constexpr int kRowThreads = 256;     // of the kernels that look twice
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kRowBlocks = 5;       // their blocks per SM
-constexpr int kKeep = 2560;          // vectors of a block that shared memory keeps (40 KB)
+constexpr int kRowBlocks = 5;        // their blocks per SM and the vectors of each that shared memory keeps (40 KB):
+constexpr int kRowKeep = 2560;       //   one tensor,
+constexpr int kPairBlocks = 4;       //   two tensors (48 KB; more registers)
+constexpr int kPairKeep = 3072;
 constexpr float kTailFloor = 1e-8f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLog2ed = 1.4426950408889634;
@@ -514,7 +515,6 @@ __device__ __forceinline__ int load_id(const Teacher& t, int64_t i, int V) {
 // the k-th largest of G >= k group maxima (a group: kThreads / G threads) is a bound that at least k values reach and few
 // others do (with k = 20 of 32 groups about 31 of independent values); what reaches it is collected and ranked by counting.
 // More than kCand (long runs of equal logits): k rounds of the smallest key above the last, which any input ends in.
-constexpr int kTopVec = 16;          // vectors per thread and unit
 constexpr int kCand = 512;
 
 struct TopScratch {
@@ -574,11 +574,11 @@ __device__ __forceinline__ void select_keys(float top, int k, int groups, TopScr
   __syncthreads();
 }
 
-template <typename T>
+template <typename T, int kTopVec>
 __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, int64_t ld, int64_t rows, int V, int k,
                                                               int groups, float kl, unsigned long long* parts,
                                                               unsigned long long* lists) {
-  constexpr int N = Vec<T>::N;
+  constexpr int N = Vec<T>::N, kHeld = kTopVec < kBatch ? kTopVec : kBatch, kBatches = kTopVec / kHeld;
   __shared__ TopScratch scratch;
   __shared__ unsigned long long warp_part[kWarps];
   const int tid = threadIdx.x;
@@ -586,12 +586,12 @@ __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, i
   const int64_t row = unit_row();
   if (row >= rows) return;
   const Slice<T> s(logits + row * ld, V, kTopVec * kThreads, blockIdx.x);
-  float m = kFloor, top[kTopVec / kBatch];
+  float m = kFloor, top[kBatches];
   Soft soft{kFloor * kl, 0.f};
 #pragma unroll
-  for (int b = 0; b < kTopVec / kBatch; ++b) {
-    uint4 x[kBatch];
-    load_unit(s, s.row, b * kBatch * kThreads, x);
+  for (int b = 0; b < kBatches; ++b) {
+    uint4 x[kHeld];
+    load_unit(s, s.row, b * kHeld * kThreads, x);
     top[b] = unit_max<T>(x);
     add_soft<T>(x, kl, m, soft);
   }
@@ -600,23 +600,23 @@ __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, i
   if ((tid & 31) == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
   float best = top[0];
 #pragma unroll
-  for (int b = 1; b < kTopVec / kBatch; ++b) best = fmaxf(best, top[b]);
+  for (int b = 1; b < kBatches; ++b) best = fmaxf(best, top[b]);
   select_keys(
       best, k, groups, scratch, lists + unit_index() * k,
       [&](float bound, auto push) {                       // few threads, and few of their vectors, get here
 #pragma unroll
-        for (int b = 0; b < kTopVec / kBatch; ++b)
+        for (int b = 0; b < kBatches; ++b)
           if (top[b] >= bound) {
-            uint4 x[kBatch];
-            load_unit(s, s.row, b * kBatch * kThreads, x);
+            uint4 x[kHeld];
+            load_unit(s, s.row, b * kHeld * kThreads, x);
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i)
+            for (int i = 0; i < kHeld; ++i)
               if (packed_max<T>(x[i]) >= bound) {
                 float f[N];
                 Vec<T>::unpack(x[i], f);
 #pragma unroll
                 for (int j = 0; j < N; ++j)
-                  if (f[j] >= bound) push(rank_key(f[j], s.start(tid + (b * kBatch + i) * kThreads) + j));
+                  if (f[j] >= bound) push(rank_key(f[j], s.start(tid + (b * kHeld + i) * kThreads) + j));
               }
           }
       },
@@ -690,8 +690,7 @@ __device__ __forceinline__ bool repeats(const int* ids, int i) {
   return r;
 }
 
-constexpr int kPartVec = 16;         // vectors per thread and unit of the loss
-constexpr int kKdVec = 8;            // the same of the gradient
+constexpr int kKdVec = 8;            // vectors per thread and unit of the gradient from statistics
 constexpr int kE = kMaxK / 32;       // teacher entries per lane: entry lane + 32 i
 
 // Lists the places in a slice of the tokens id[0 .. kE) over one warp; returns their number.
@@ -840,7 +839,7 @@ __device__ __forceinline__ uint4 scaled_exp(const uint4& x, Two scale, Two minus
 }
 
 // The tail's part of one unit: vectors that hold a teacher's token give it up.
-template <typename T>
+template <typename T, int kPartVec>
 __global__ void __launch_bounds__(kThreads) kd_parts_kernel(const T* logits, int64_t ld, int64_t rows, int V, Teacher t,
                                                             float kl, unsigned long long* parts) {
   constexpr int N = Vec<T>::N;
@@ -890,6 +889,7 @@ __global__ void __launch_bounds__(32) kd_loss_kernel(const T* logits, int64_t ld
                                                      const unsigned long long* parts, float* loss, KdRow* stats) {
   __shared__ int s_id[kMaxK];
   const int64_t row = blockIdx.x;
+  pdl_launch_dependents();
   int id[kE];
   load_ids(t, row, V, id);
   float lp[kE], z[kE];
@@ -1065,7 +1065,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) kd_grad_kernel(const 
     if (s.owns(list.id[j]) || list.id[j] == single) o[list.id[j]] = Vec<T>::back(kd_pull(f, w, list.z[j], list.pt[j], kl));
 }
 
-// The gradient from saved statistics.
+// The gradient from statistics, elementwise; `out` may be the logits.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64_t ld, int64_t rows, int V, Teacher t,
                                                           float kl, float inv_t, const float* weight,
@@ -1075,18 +1075,22 @@ __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64
   const Slice<T> s(logits + row * ld, V, kKdVec * kThreads, blockIdx.x);
   uint4 x[kKdVec];
   load_unit(s, x);
+  T* o = out + row * out_ld;
+  const int tid = threadIdx.x;
+  int id = tid < t.k ? load_id(t, row * t.k + tid, V) : -1;
+  if (id >= 0 && s.place(id) < 0) id = -1;
+  const float z = id >= 0 ? masked(Vec<T>::one(s.row[id])) : 0.f;
+  pdl_wait();
   const KdRow st = stats[row];
   const float w = st.inv_s == 0.f ? 0.f : weight[row] * inv_t;
-  T* o = out + row * out_ld;
-  const int tid = threadIdx.x, id = tid < t.k ? load_id(t, row * t.k + tid, V) : -1;
   const Two scale = two(st.inv_s == 0.f ? 0.f : -st.csum * st.inv_s * w), c2 = two(-st.c), k2 = two(kl);
+  __syncthreads();                                     // every z is read
   store_unit<kKdVec>(s, o, [&](int i) { return scaled_exp<T>(x[i], scale, c2, k2); });
   __syncthreads();
-  if (id >= 0 && s.place(id) >= 0) {
+  if (id >= 0) {
     bool repeated = false;
     for (int j = 0; j < tid; ++j) repeated |= load_id(t, row * t.k + j, V) == id;
-    const float pt = expf(t.lp[row * t.k + tid]);
-    if (!repeated) o[id] = Vec<T>::back(kd_pull(st, w, masked(Vec<T>::one(s.row[id])), pt, kl));
+    if (!repeated) o[id] = Vec<T>::back(kd_pull(st, w, z, expf(t.lp[row * t.k + tid]), kl));
   }
 }
 
@@ -1181,7 +1185,7 @@ __device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&
 
 // One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p).
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads, kRowBlocks) accept_kernel(const T* draft, int64_t ldq, const T* target,
+__global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const T* draft, int64_t ldq, const T* target,
                                                                          int64_t ldp, int V, int keep, float kl, float temp,
                                                                          float* alpha, float* out_kl, AcceptRow* stats) {
   constexpr int N = Vec<T>::N;
@@ -1352,11 +1356,21 @@ constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr int kDrawVec = 2;          // vectors that a thread requests at once
 
 constexpr uint64_t kIndexStep = 0x8CB92BA72F3D8DD7ull;
-// The sampler's 23 random bits of counter base + index kIndexStep.
-__device__ __forceinline__ uint32_t random23(uint64_t z) {
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-  return (uint32_t)(z >> 32) >> 9;     // the last step, z ^ (z >> 31), leaves bits 33 and up as they are
+// x * c modulo 2^64 in 32-bit halves
+__device__ __forceinline__ uint2 mul64(uint32_t lo, uint32_t hi, uint64_t c) {
+  const uint64_t w = (uint64_t)lo * (uint32_t)c;
+  return make_uint2((uint32_t)w, (uint32_t)(w >> 32) + lo * (uint32_t)(c >> 32) + hi * (uint32_t)c);
+}
+// The sampler's 23 random bits of counter base + index kIndexStep: z ^= z >> 30, z *= c1, z ^= z >> 27, z *= c2, and the top
+// bits, which its last step, z ^ (z >> 31), leaves as they are.
+__device__ __forceinline__ uint32_t random23(uint64_t counter) {
+  uint32_t lo = (uint32_t)counter, hi = (uint32_t)(counter >> 32);
+  lo ^= __funnelshift_r(lo, hi, 30);
+  hi ^= hi >> 30;
+  const uint2 y = mul64(lo, hi, 0xBF58476D1CE4E5B9ull);
+  lo = y.x ^ __funnelshift_r(y.x, y.y, 27);
+  hi = y.y ^ (y.y >> 27);
+  return mul64(lo, hi, 0x94D049BB133111EBull).y >> 9;
 }
 __device__ __forceinline__ float unit(uint32_t h) { return ((float)h + 0.5f) * (1.0f / 8388608.0f); }
 
@@ -1372,7 +1386,7 @@ __device__ __forceinline__ unsigned long long* verify_best(const Verify& a) {
 __device__ __forceinline__ unsigned long long* verify_count(const Verify& a) { return verify_best(a) + a.batch; }
 __device__ __forceinline__ unsigned long long* verify_parts(const Verify& a) { return verify_best(a) + 2 * a.batch; }
 
-template <typename T, int kUnroll>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int splits) {
   constexpr int N = Vec<T>::N;
   __shared__ unsigned long long warp_part[kWarps];
@@ -1391,8 +1405,8 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
   if ((draft ? j - a.k - 1 >= n : j > n) || (draft && greedy)) return;
   const T* row = draft ? static_cast<const T*>(a.draft_logits) + b * a.draft_b + (j - a.k - 1) * a.draft_j
                        : static_cast<const T*>(a.logits) + b * a.logits_b + j * a.logits_j;
-  const Slice<T> s(row, a.V, kUnroll * kThreads, split);
-  uint4 x[kUnroll];
+  const Slice<T> s(row, a.V, kBatch * kThreads, split);
+  uint4 x[kBatch];
   load_unit(s, x);
   const float top = unit_max<T>(x);
   unsigned long long res;
@@ -1401,7 +1415,7 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
     const float best = warp_reduce(top, Max());
     if (top == best && best >= kFloor) {
 #pragma unroll
-      for (int i = kUnroll - 1; i >= 0; --i) {          // ends at the thread's first element of that value
+      for (int i = kBatch - 1; i >= 0; --i) {          // ends at the thread's first element of that value
         float f[N];
         Vec<T>::unpack(x[i], f);
 #pragma unroll
@@ -1459,16 +1473,7 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
       }
       continue;
     }
-    const auto whole = [&](int r) {
-      Soft t{kFloor * kl, 0.f};
-      for (int i = lane; i < splits; i += 32) {
-        const unsigned long long w = parts[r * splits + i];
-        t = join(t, Soft{__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))});
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) t = join(t, shfl_xor(t, o));
-      return t;
-    };
+    const auto whole = [&](int r) { return join_parts(splits, kl, [&](int i) { return parts[r * splits + i]; }); };
     const Soft p = whole(j), q = a.draft_logits && j < n ? whole(a.k + 1 + j) : Soft{0.f, 1.f};
     if (lane == 0) {
       s_p[j] = p;
@@ -1505,67 +1510,86 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
   const float ip = 1.f / p.sum, cq = qrow ? s_q[acc].c : 0.f, iq = qrow && s_q[acc].sum > 0.f ? 1.f / s_q[acc].sum : 0.f;
   const bool same = ((reinterpret_cast<uintptr_t>(qrow) ^ reinterpret_cast<uintptr_t>(row)) & 15) == 0;
   const uint64_t base = seed + (step + acc) * 0xD1B54A32D192ED03ull;
-  // The block that completes a sequence finds an empty residual, and then draws from p itself, all of the row alone.
-  for (int whole = acc == n, mine = 1;; whole = 1, mine = 0) {
-    const Slice<T> s(row, a.V, mine ? per : a.V, mine ? rank : 0);
+  // The earliest of all times is exponential with the rate sum r: 1 for p, 1 - p(d) beside a point mass. A draw that only
+  // looks for times up to 24 / rate misses them in one of 2^34 cases, and what it saves is the logarithms that each warp
+  // took until it had a bound of its own (39 us to XX us for 64 residuals of 151936 bf16 tokens). The rate of a residual is
+  // not known; 1024 covers all but rates of 1/64 and below, which are rejected as rarely. The block that completes a
+  // sequence without a token repeats the search alone, without the limit, and, if the residual is empty, over p itself.
+  float limit = 24.f;
+  if (qrow) limit = 1024.f;
+  else if (id >= 0 && id < a.V) limit = 24.f / fmaxf(1.f - ex2(fmaf(Vec<T>::one(row[id]), kl, -p.c)) * ip, 1e-6f);
+  for (int stage = 0;; ++stage) {
+    const bool whole = acc == n || stage == 2;
+    const Slice<T> s(row, a.V, stage ? a.V : per, stage ? 0 : rank);
     unsigned long long best = kNone;
-    float bound = INFINITY;                                           // of this warp: its best time, rounded up
-    for (int v0 = tid; v0 - lane < s.count; v0 += kDrawVec * kDrawThreads) {   // the same trip count for a whole warp
-      uint4 xp[kDrawVec], xq[kDrawVec];
+    float bound = stage ? INFINITY : limit;                           // of this warp: the limit, then its best time
+    const auto race = [&](auto residual) {                            // 0: p, 1: p without the draft, 2: p - q
+      for (int v0 = tid; v0 - lane < s.count; v0 += kDrawVec * kDrawThreads) {   // the same trip count for a whole warp
+        uint4 xp[kDrawVec], xq[kDrawVec];
 #pragma unroll
-      for (int i = 0; i < kDrawVec; ++i) {
-        const int v = v0 + i * kDrawThreads, i0 = s.start(v);
-        xp[i] = xq[i] = make_uint4(Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad);
-        if (v < s.count) {
-          xp[i] = s.full(i0) ? __ldcs(reinterpret_cast<const uint4*>(row + i0)) : ragged_vec(s, row, i0);
-          if (qrow && !whole)
-            xq[i] = same && s.full(i0) ? __ldcs(reinterpret_cast<const uint4*>(qrow + i0)) : ragged_vec(s, qrow, i0);
+        for (int i = 0; i < kDrawVec; ++i) {
+          const int v = v0 + i * kDrawThreads, i0 = s.start(v);
+          xp[i] = xq[i] = make_uint4(Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad, Vec<T>::kPad);
+          if (v < s.count) {
+            xp[i] = s.full(i0) ? __ldcs(reinterpret_cast<const uint4*>(row + i0)) : ragged_vec(s, row, i0);
+            if (residual == 2)
+              xq[i] = same && s.full(i0) ? __ldcs(reinterpret_cast<const uint4*>(qrow + i0)) : ragged_vec(s, qrow, i0);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kDrawVec; ++i) {
+          if (v0 - lane + i * kDrawThreads >= s.count) break;          // for the whole warp
+          const int i0 = s.start(v0 + i * kDrawThreads);
+          float f[N], g[N];
+          Vec<T>::unpack(xp[i], f);
+          Vec<T>::unpack(xq[i], g);
+          uint64_t counter = base + (uint64_t)(int64_t)i0 * kIndexStep;
+#pragma unroll
+          for (int k0 = 0; k0 < N; k0 += 4) {                         // one branch for four tokens
+            float r[4], ahead = 1.f;
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k, counter += kIndexStep) {
+              r[k] = ex2(fmaf(f[k0 + k], kl, -p.c)) * ip;
+              if (residual == 1 && i0 + k0 + k == id) r[k] = 0.f;
+              if (residual == 2) r[k] = fmaf(ex2(fmaf(g[k0 + k], kl, -cq)), -iq, r[k]);
+              // u = (h + 1/2) 2^-23; -log(u) > 1 - u > 1 - (h + 1) 2^-23, exact from 1 + h 2^-23
+              h[k] = random23(counter);
+              const float miss = (2.f - 0x1p-23f) - __uint_as_float(0x3F800000u | h[k]);
+              ahead = fminf(ahead, fmaf(-bound, r[k], miss));         // above 0 for r <= 0, no operand where it is NaN
+            }
+            if (ahead <= 0.f)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float e = -logf(unit(h[k])) / r[k];
+                if (r[k] > 0.f && e <= bound) {
+                  best = min(best, (unsigned long long)__float_as_uint(e) << 32 | (uint32_t)(i0 + k0 + k));
+                  bound = e * 1.000001f;                              // rounded up: ties stay in
+                }
+              }
+          }
+          bound = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(bound)));
         }
       }
-#pragma unroll
-      for (int i = 0; i < kDrawVec; ++i) {
-        if (v0 - lane + i * kDrawThreads >= s.count) break;            // for the whole warp
-        const int i0 = s.start(v0 + i * kDrawThreads);
-        float f[N], g[N];
-        Vec<T>::unpack(xp[i], f);
-        Vec<T>::unpack(xq[i], g);
-        uint64_t counter = base + (uint64_t)(int64_t)i0 * kIndexStep;
-#pragma unroll
-        for (int k = 0; k < N; ++k, counter += kIndexStep) {
-          float r = ex2(fmaf(f[k], kl, -p.c)) * ip;
-          if (!whole) {
-            if (qrow) r = fmaf(ex2(fmaf(g[k], kl, -cq)), -iq, r);
-            else if (i0 + k == id) r = 0.f;
-          }
-          // u = (h + 1/2) 2^-23 and 1 - u, from the fraction bits h of 1 + h 2^-23; -log(u) > 1 - u
-          const uint32_t h = random23(counter);
-          const float miss = (2.f - __uint_as_float(0x3F800000u | h)) - 0x1p-24f;
-          if (miss <= bound * r) {                                    // false for r <= 0, and where r is NaN
-            const float e = -logf(unit(h)) / r;
-            best = min(best, (unsigned long long)__float_as_uint(e) << 32 | (uint32_t)(i0 + k));
-            bound = fminf(bound, e * 1.000001f);
-          }
-          if (k == 0 || k == N / 2)                                   // early, or a warp's first vector takes all logarithms
-            bound = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(bound)));
-        }
-        bound = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(bound)));
-      }
-    }
+    };
+    if (whole) race(std::integral_constant<int, 0>());
+    else if (qrow) race(std::integral_constant<int, 2>());
+    else race(std::integral_constant<int, 1>());
     best = warp_reduce(best, MinKey());
     if (lane == 0) warp_best[tid >> 5] = best;
     __syncthreads();
     if (tid == 0) {
       for (int i = 1; i < kDrawWarps; ++i) best = min(best, warp_best[i]);
       s_again = false;
-      bool last = !mine;
-      if (mine) {
+      bool last = stage > 0;
+      if (!stage) {
         atomicMin(verify_best(a) + b, best);
         __threadfence();
         last = atomicAdd(verify_count(a) + b, 1ull) == (unsigned long long)(blocks - 1);
         if (last) best = atomicMin(verify_best(a) + b, kNone);
       }
       if (last) {
-        s_again = best == kNone && !whole;
+        s_again = best == kNone && stage < (acc == n ? 1 : 2) && p.sum > 0.f;
         a.accepted[b] = acc;
         a.next[b] = best == kNone ? -1 : (int)(uint32_t)best;
       }
@@ -1589,19 +1613,18 @@ int splits_of(Type type, Logits z, int64_t rows, int V, int unit) {
   return ((V + lanes - 1) / lanes + (aligned ? 0 : 1) + unit - 1) / unit;
 }
 
-// Blocks per row (a cluster) and vectors that a block keeps, in the kernels that look twice; `sides` tensors share a block.
+// Blocks per row (a cluster) and vectors of each tensor that a block keeps, in the kernels that look twice; `sides` tensors
+// share a block.
 struct Plan {
   int cluster, keep, smem;
 };
 Plan plan_of(Type type, int64_t rows, int V, int sides) {
-  const int total = V / (type == F32 ? 4 : 8) + 1;
-  const int64_t slots = kRowBlocks * sm_count();
-  // enough blocks per row that what all running blocks do not keep stays in half of L2, then as few as leave no more than
-  // a seventh of the slots idle over all waves
+  const int total = V / (type == F32 ? 4 : 8) + 1, held = sides == 1 ? kRowKeep : kPairKeep;
+  const int64_t slots = (sides == 1 ? kRowBlocks : kPairBlocks) * sm_count();
   int c = 1;
-  while (c < kMaxCluster && (total * sides / c - kKeep) * 16ll * slots > 64 << 20) c *= 2;
-  while (c < kMaxCluster && total * sides > kRowThreads * c && rows * c * 7 < (rows * c + slots - 1) / slots * slots * 6) c *= 2;
-  const int per = (total + c - 1) / c, keep = std::min(per, kKeep / sides) / kRound * kRound;
+  while (c < kMaxCluster && (total * sides / c - held) * 16ll * slots > 64 << 20) c *= 2;
+  while (c < kMaxCluster && total * sides > kRowThreads * c && rows * c * 2 <= slots) c *= 2;
+  const int per = (total + c - 1) / c, keep = std::min(per, held / sides) / kRound * kRound;
   return {c, keep, keep * sides * 16};
 }
 
@@ -1693,12 +1716,16 @@ KdRows carve_kd(int64_t rows, int k, void* p, size_t& bytes) {
 
 }  // namespace
 
+// Vectors per thread and unit of top-k
+static int top_vec(Type type, Logits z, int64_t rows, int V) {
+  return type == F32 && rows * splits_of(type, z, rows, V, 16 * kThreads) >= 2 * sm_count() ? 16 : 8;
+}
 size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V, int k) {
-  return carve_topk(rows * splits_of(type, z, rows, V, kTopVec * kThreads), k, nullptr).bytes;
+  return carve_topk(rows * splits_of(type, z, rows, V, top_vec(type, z, rows, V) * kThreads), k, nullptr).bytes;
 }
 cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float temp, int32_t* ids, float* lp,
                          void* workspace, cudaStream_t stream) {
-  const int splits = splits_of(type, z, rows, V, kTopVec * kThreads);
+  const int vec = top_vec(type, z, rows, V), splits = splits_of(type, z, rows, V, vec * kThreads);
   const TopWork w = carve_topk(rows * splits, k, workspace);
   const int groups = k <= 24 ? 32 : k <= 48 ? 64 : k <= 96 ? 128 : 256;
   Shape units, merge;
@@ -1707,19 +1734,28 @@ cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float 
   merge.early = true;
   const cudaError_t e = by_type(type, [&](auto t) {
     using T = decltype(t);
-    return launch(topk_units_kernel<T>, units, stream, static_cast<const T*>(z.p), z.ld, rows, V, k, groups, (float)(kLog2ed / temp),
-                  w.parts, w.lists);
+    const auto go = [&](auto kernel) {
+      return launch(kernel, units, stream, static_cast<const T*>(z.p), z.ld, rows, V, k, groups, (float)(kLog2ed / temp),
+                    w.parts, w.lists);
+    };
+    if constexpr (sizeof(T) == 4)
+      if (vec == 16) return go(topk_units_kernel<T, 16>);
+    return go(topk_units_kernel<T, 8>);
   });
   if (e != cudaSuccess) return e;
   return launch(topk_merge_kernel, merge, stream, splits, k, groups, (float)(kLog2ed / temp), w.parts, w.lists, ids, lp);
 }
 
+// Vectors per thread and unit of the tail sums
+static int part_vec(Type type, Logits z, int64_t rows, int V) {
+  return type != F32 && rows * splits_of(type, z, rows, V, 16 * kThreads) >= 2 * sm_count() ? 16 : 8;
+}
 size_t kd_topk_loss_workspace(Type type, Logits z, int64_t rows, int V) {
-  return rows * splits_of(type, z, rows, V, kPartVec * kThreads) * sizeof(unsigned long long);
+  return rows * splits_of(type, z, rows, V, part_vec(type, z, rows, V) * kThreads) * sizeof(unsigned long long);
 }
 cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, float* loss, float* stats,
                          void* workspace, cudaStream_t stream) {
-  const int splits = splits_of(type, z, rows, V, kPartVec * kThreads);
+  const int vec = part_vec(type, z, rows, V), splits = splits_of(type, z, rows, V, vec * kThreads);
   unsigned long long* words = static_cast<unsigned long long*>(workspace);
   Shape parts, last;
   parts.blocks = last.blocks = rows;
@@ -1729,19 +1765,50 @@ cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, fl
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     const T* p = static_cast<const T*>(z.p);
-    const cudaError_t e = launch(kd_parts_kernel<T>, parts, stream, p, z.ld, rows, V, t, (float)(kLog2ed / temp), words);
+    const auto go = [&](auto kernel) {
+      return launch(kernel, parts, stream, p, z.ld, rows, V, t, (float)(kLog2ed / temp), words);
+    };
+    cudaError_t e;
+    if constexpr (sizeof(T) == 4) e = go(kd_parts_kernel<T, 8>);
+    else e = vec == 16 ? go(kd_parts_kernel<T, 16>) : go(kd_parts_kernel<T, 8>);
     if (e != cudaSuccess) return e;
     return launch(kd_loss_kernel<T>, last, stream, p, z.ld, splits, V, t, (float)(kLog2ed / temp), words, loss,
                   reinterpret_cast<KdRow*>(stats));
   });
 }
-size_t kd_topk_grad_workspace(int64_t rows, int k) {
+
+static cudaError_t kd_from_stats(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
+                                 const float* stats, void* out, int64_t out_ld, bool early, cudaStream_t stream) {
+  Shape s;
+  s.blocks = rows;
+  s.units = splits_of(type, z, rows, V, kKdVec * kThreads);
+  s.early = early;
+  return by_type(type, [&](auto x) {
+    using T = decltype(x);
+    return launch(kd_bwd_kernel<T>, s, stream, static_cast<const T*>(z.p), z.ld, rows, V, t, (float)(kLog2ed / temp),
+                  1.f / temp, weight, reinterpret_cast<const KdRow*>(stats), static_cast<T*>(out), out_ld);
+  });
+}
+
+// Logits that fit in L2 are read from there the second time whichever block does it
+static bool kd_in_l2(Type type, int64_t rows, int V) {
+  int dev = 0, l2 = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&l2, cudaDevAttrL2CacheSize, dev) != cudaSuccess) return false;
+  return rows * V * (type == F32 ? 4 : 2) <= l2;
+}
+size_t kd_topk_grad_workspace(Type type, Logits z, int64_t rows, int V, int k) {
+  if (kd_in_l2(type, rows, V)) return rows * sizeof(KdRow) + kd_topk_loss_workspace(type, z, rows, V);
   size_t bytes;
   carve_kd(rows, k, nullptr, bytes);
   return bytes;
 }
 cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
                          float* loss, void* out, int64_t out_ld, void* workspace, cudaStream_t stream) {
+  if (kd_in_l2(type, rows, V)) {
+    float* stats = static_cast<float*>(workspace);
+    const cudaError_t e = kd_topk_loss(type, z, rows, V, t, temp, loss, stats, stats + rows * kKdStats, stream);
+    return e != cudaSuccess ? e : kd_from_stats(type, z, rows, V, t, temp, weight, stats, out, out_ld, true, stream);
+  }
   size_t bytes;
   const KdRows r = carve_kd(rows, t.k, workspace, bytes);
   const Plan p = plan_of(type, rows, V, 1);
@@ -1764,14 +1831,7 @@ cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, fl
 }
 cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
                         const float* stats, void* out, int64_t out_ld, cudaStream_t stream) {
-  Shape s;
-  s.blocks = rows;
-  s.units = splits_of(type, z, rows, V, kKdVec * kThreads);
-  return by_type(type, [&](auto x) {
-    using T = decltype(x);
-    return launch(kd_bwd_kernel<T>, s, stream, static_cast<const T*>(z.p), z.ld, rows, V, t, (float)(kLog2ed / temp), 1.f / temp, weight,
-                  reinterpret_cast<const KdRow*>(stats), static_cast<T*>(out), out_ld);
-  });
+  return kd_from_stats(type, z, rows, V, t, temp, weight, stats, out, out_ld, false, stream);
 }
 
 cudaError_t accept_kl(Type type, Logits draft, Logits target, int64_t rows, int V, float temp, float* alpha, float* kl,
@@ -1803,14 +1863,11 @@ cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, 
 
 namespace {
 struct VerifyPlan {
-  int unroll, splits, rows;
+  int splits, rows;            // units per row; rows per sequence
 };
 VerifyPlan verify_plan(const Verify& a) {
   const int lanes = a.type == F32 ? 4 : 8, total = (a.V + lanes - 1) / lanes + 1;
-  const int rows = a.draft_logits ? 2 * a.k + 1 : a.k + 1;
-  const auto splits = [&](int unroll) { return (total + unroll * kThreads - 1) / (unroll * kThreads); };
-  const int unroll = a.batch * rows * splits(8) >= 2 * sm_count() ? 8 : 2;
-  return {unroll, splits(unroll), rows};
+  return {(total + kBatch * kThreads - 1) / (kBatch * kThreads), a.draft_logits ? 2 * a.k + 1 : a.k + 1};
 }
 }  // namespace
 
@@ -1825,12 +1882,11 @@ cudaError_t spec_verify(const Verify& a, cudaStream_t stream) {
     using T = decltype(x);
     Shape parts, draw;
     parts.blocks = a.batch * p.rows * p.splits;
-    cudaError_t e = launch(p.unroll == 8 ? verify_parts_kernel<T, 8> : verify_parts_kernel<T, 2>, parts, stream, a,
-                           p.splits);
+    const cudaError_t e = launch(verify_parts_kernel<T>, parts, stream, a, p.splits);
     if (e != cudaSuccess) return e;
-    // four blocks per SM over all sequences, each of at least one vector per thread
+    // as many blocks as run at once over all sequences, each of at least one vector per thread
     const int total = (a.V + Vec<T>::N - 1) / Vec<T>::N + 1;
-    const int64_t most = (total + kDrawThreads - 1) / kDrawThreads, want = (4 * sm_count() + a.batch - 1) / a.batch;
+    const int64_t most = (total + kDrawThreads - 1) / kDrawThreads, want = std::max<int64_t>(1, (5 * sm_count()) / a.batch);
     const int c = (int)std::min(most, want);
     draw.blocks = a.batch * c;
     draw.threads = kDrawThreads;

@@ -36,7 +36,7 @@ size_t kd_topk_loss_workspace(Type type, Logits z, int64_t rows, int V);
 cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, float* loss, float* stats,
                          void* workspace, cudaStream_t stream);
 // loss, and out = d sum(weight loss) / d logits; out may be the logits
-size_t kd_topk_grad_workspace(int64_t rows, int k);
+size_t kd_topk_grad_workspace(Type type, Logits z, int64_t rows, int V, int k);
 cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
                          float* loss, void* out, int64_t out_ld, void* workspace, cudaStream_t stream);
 cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,
