@@ -465,9 +465,9 @@ __device__ __forceinline__ float unit_max(const uint4 (&x)[kVec]) {
     return fmaxf(Vec<T>::one(m.x), Vec<T>::one(m.y));
   }
 }
-// Adds vectors to a thread's running softmax with maximum m.
+// Adds vectors to a thread's running softmax with maximum m; returns their largest logit.
 template <typename T, int kVec>
-__device__ __forceinline__ void add_soft(const uint4 (&x)[kVec], float kl, float& m, Soft& s) {
+__device__ __forceinline__ float add_soft(const uint4 (&x)[kVec], float kl, float& m, Soft& s) {
   constexpr int N = Vec<T>::N;
   const float vm = unit_max<T>(x);
   if (vm > m) {
@@ -489,6 +489,7 @@ __device__ __forceinline__ void add_soft(const uint4 (&x)[kVec], float kl, float
     }
   }
   s.sum += sum(add2(a, b));
+  return vm;
 }
 // Joins a list of parts over a warp, in an order that depends on their number alone: every lane gets the same bits.
 template <typename Load>
@@ -511,169 +512,146 @@ __device__ __forceinline__ int load_id(const Teacher& t, int64_t i, int V) {
 }
 
 // ------------------------------------------------------------------------------------------- teacher top-k
-// Each unit yields its k best keys in order; a second kernel selects the k best of a row's lists the same way. Selection:
-// the k-th largest of G >= k group maxima (a group: kThreads / G threads) is a bound that at least k values reach and few
-// others do (with k = 20 of 32 groups about 31 of independent values); what reaches it is collected and ranked by counting.
-// More than kCand (long runs of equal logits): k rounds of the smallest key above the last, which any input ends in.
+// The first kernel reads the logits: softmax parts, and the maximum of each thread's vectors. The second, one block per row,
+// selects: the k-th largest of G >= k group maxima (a group: the logits of kThreads / G threads over all units) is a bound
+// that at least k values reach and few others do (with k = 20 of 32 groups about 31 of independent values). The vectors
+// of threads whose maximum reaches it are read again, one per thread; what reaches it is collected and ranked by counting. More than kCand
+// (long runs of equal logits): k rounds of the smallest key above the last, which any input ends in.
 constexpr int kCand = 512;
 
-struct TopScratch {
-  unsigned long long cand[kCand], warp[kWarps];
-  float gmax[kThreads];
-  float bound;
-  int count;
-};
-
-// The k smallest keys of the block, ascending, to out[0 .. k) (kNone where there are fewer). `top`: the calling thread's
-// largest value (below kFloor: none); collect(bound, push) calls push(key) for its keys of values >= bound; after(last)
-// is its smallest key above `last`. `groups` as above. Begins and ends behind a barrier.
-template <typename Collect, typename After>
-__device__ __forceinline__ void select_keys(float top, int k, int groups, TopScratch& s, unsigned long long* out,
-                                            Collect collect, After after) {
-  const int tid = threadIdx.x, shift = __ffs(kThreads / groups) - 1;
-  float g = top;
-  for (int o = (1 << shift) >> 1; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-  if ((tid & ((1 << shift) - 1)) == 0) s.gmax[tid >> shift] = g;
-  if (tid == 0) s.count = 0;
-  __syncthreads();
-  if (tid < groups) {
-    g = s.gmax[tid];
-    int r = 0;
-    for (int j = 0; j < groups; ++j) r += s.gmax[j] > g || (s.gmax[j] == g && j < tid);
-    if (r == k - 1) s.bound = fmaxf(g, kFloor);   // kFloor: fewer than k groups hold a value, and all are collected
-  }
-  __syncthreads();
-  const float bound = s.bound;
-  if (top >= bound)
-    collect(bound, [&](unsigned long long key) {
-      const int at = atomicAdd(&s.count, 1);
-      if (at < kCand) s.cand[at] = key;
-    });
-  __syncthreads();
-  const int n = s.count;
-  if (n <= kCand) {
-    for (int i = tid; i < n; i += kThreads) {
-      const unsigned long long key = s.cand[i];
-      int r = 0;
-      for (int j = 0; j < n; ++j) r += s.cand[j] < key;
-      if (r < k) out[r] = key;
-    }
-    for (int i = n + tid; i < k; i += kThreads) out[i] = kNone;
-  } else {
-    unsigned long long last = 0;     // below every key of an unmasked logit
-    for (int j = 0; j < k; ++j) {
-      unsigned long long b = warp_reduce(after(last), MinKey());
-      __syncthreads();
-      if ((tid & 31) == 0) s.warp[tid >> 5] = b;
-      __syncthreads();
-      for (int w = 0; w < kWarps; ++w) b = min(b, s.warp[w]);
-      if (tid == 0) out[j] = b;
-      last = b;
-    }
-  }
-  __syncthreads();
-}
-
-template <typename T, int kTopVec>
-__global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, int64_t ld, int64_t rows, int V, int k,
-                                                              int groups, float kl, unsigned long long* parts,
-                                                              unsigned long long* lists) {
-  constexpr int N = Vec<T>::N, kHeld = kTopVec < kBatch ? kTopVec : kBatch, kBatches = kTopVec / kHeld;
-  __shared__ TopScratch scratch;
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, int64_t ld, int64_t rows, int V, float kl,
+                                                              unsigned long long* parts, float* tops) {
   __shared__ unsigned long long warp_part[kWarps];
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   const int64_t row = unit_row();
   if (row >= rows) return;
-  const Slice<T> s(logits + row * ld, V, kTopVec * kThreads, blockIdx.x);
-  float m = kFloor, top[kBatches];
+  const Slice<T> s(logits + row * ld, V, kVec * kThreads, blockIdx.x);
+  float m = kFloor, top = -INFINITY;
   Soft soft{kFloor * kl, 0.f};
 #pragma unroll
-  for (int b = 0; b < kBatches; ++b) {
-    uint4 x[kHeld];
-    load_unit(s, s.row, b * kHeld * kThreads, x);
-    top[b] = unit_max<T>(x);
-    add_soft<T>(x, kl, m, soft);
+  for (int b = 0; b < kVec / kBatch; ++b) {
+    uint4 x[kBatch];
+    load_unit(s, s.row, b * kBatch * kThreads, x);
+    top = fmaxf(top, add_soft<T>(x, kl, m, soft));
   }
+  tops[unit_index() * kThreads + tid] = top;
 #pragma unroll
   for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
   if ((tid & 31) == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
-  float best = top[0];
-#pragma unroll
-  for (int b = 1; b < kBatches; ++b) best = fmaxf(best, top[b]);
-  select_keys(
-      best, k, groups, scratch, lists + unit_index() * k,
-      [&](float bound, auto push) {                       // few threads, and few of their vectors, get here
-#pragma unroll
-        for (int b = 0; b < kBatches; ++b)
-          if (top[b] >= bound) {
-            uint4 x[kHeld];
-            load_unit(s, s.row, b * kHeld * kThreads, x);
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i)
-              if (packed_max<T>(x[i]) >= bound) {
-                float f[N];
-                Vec<T>::unpack(x[i], f);
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                  if (f[j] >= bound) push(rank_key(f[j], s.start(tid + (b * kHeld + i) * kThreads) + j));
-              }
-          }
-      },
-      [&](unsigned long long last) {
-        unsigned long long b = kNone;
-        for (int v = tid; v < s.count; v += kThreads)
-          for (int j = 0; j < N; ++j) {
-            const int at = s.start(v) + j;
-            if (at < 0 || at >= V) continue;
-            const float z = Vec<T>::one(s.row[at]);
-            const unsigned long long key = rank_key(z, at);
-            if (z >= kFloor && key > last && key < b) b = key;
-          }
-        return b;
-      });
+  __syncthreads();
   if (tid < 32) {
     const Soft t = join_parts(kWarps, kl, [&](int i) { return warp_part[i]; });
     if (tid == 0) parts[unit_index()] = as_u64(t.c, t.sum);
   }
 }
 
-__global__ void __launch_bounds__(kThreads) topk_merge_kernel(int splits, int k, int groups, float kl,
-                                                              const unsigned long long* parts,
-                                                              const unsigned long long* lists, int32_t* ids, float* lp) {
-  __shared__ TopScratch scratch;
-  __shared__ unsigned long long mine[kMaxK];
-  __shared__ float s_soft[2];
-  const int tid = threadIdx.x;
+// `vec`: vectors per thread and unit of the first kernel
+template <typename T>
+__global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, int64_t ld, int V, int vec, int units, int k,
+                                                               int groups, float kl, const unsigned long long* parts,
+                                                               const float* tops, int32_t* ids, float* lp) {
+  constexpr int N = Vec<T>::N;
+  __shared__ unsigned long long cand[kCand], warp_key[kWarps];
+  __shared__ float gmax[kThreads], s_bound, s_soft[2];
+  __shared__ int list[kCand], s_listed, s_count;
+  const int tid = threadIdx.x, shift = __ffs(kThreads / groups) - 1;
   const int64_t row = blockIdx.x;
+  const Slice<T> s(logits + row * ld, V, V + N, 0);
+  tops += row * units * kThreads + tid;
   pdl_wait();
-  if (tid < 32) {
-    const Soft t = join_parts(splits, kl, [&](int i) { return parts[row * splits + i]; });
-    if (tid == 0) {
+  const auto each_top = [&](auto f) {              // f(unit, maximum) for this thread of every unit
+    for (int u0 = 0; u0 < units; u0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = u0 + i < units ? tops[(u0 + i) * kThreads] : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f(u0 + i, x[i]);
+    }
+  };
+  float top = -INFINITY;
+  each_top([&](int, float x) { top = fmaxf(top, x); });
+  float g = top;
+  for (int o = (1 << shift) >> 1; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if ((tid & ((1 << shift) - 1)) == 0) gmax[tid >> shift] = g;
+  if (tid == 0) s_listed = s_count = 0;
+  __syncthreads();
+  if (tid < groups) {
+    g = gmax[tid];
+    int r = 0;
+    for (int j = 0; j < groups; ++j) r += gmax[j] > g || (gmax[j] == g && j < tid);
+    if (r == k - 1) s_bound = fmaxf(g, kFloor);    // kFloor: fewer than k groups hold a value, and all are collected
+  }
+  if (tid >= kThreads - 32) {
+    const Soft t = join_parts(units, kl, [&](int i) { return parts[row * units + i]; });
+    if (tid == kThreads - 1) {
       s_soft[0] = t.c;
       s_soft[1] = log2f(t.sum);
     }
   }
-  const unsigned long long* keys = lists + row * splits * k;
-  const int n = splits * k;
-  unsigned long long first = kNone;
-  for (int i = tid; i < n; i += kThreads) first = min(first, keys[i]);
-  select_keys(
-      first == kNone ? -INFINITY : key_value(first), k, groups, scratch, mine,
-      [&](float bound, auto push) {
-        for (int i = tid; i < n; i += kThreads)
-          if (keys[i] != kNone && key_value(keys[i]) >= bound) push(keys[i]);
-      },
-      [&](unsigned long long last) {
-        unsigned long long b = kNone;
-        for (int i = tid; i < n; i += kThreads)
-          if (keys[i] > last && keys[i] < b) b = keys[i];
-        return b;
+  __syncthreads();
+  const float bound = s_bound;
+  if (top >= bound)
+    each_top([&](int u, float x) {
+      if (x >= bound) {
+        const int at = atomicAdd(&s_listed, 1);
+        if (at < kCand) list[at] = u << 8 | tid;
+      }
+    });
+  __syncthreads();
+  // visits the logits that reach the bound in vector i of the thread and unit `from`
+  const auto look = [&](int from, int i, auto visit) {
+    const int at = s.start(((from >> 8) * vec + i) * kThreads + (from & 255));
+    const uint4 x = s.full(at) ? __ldcg(reinterpret_cast<const uint4*>(s.row + at)) : ragged_vec(s, s.row, at);
+    if (packed_max<T>(x) >= bound) {
+      float f[N];
+      Vec<T>::unpack(x, f);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (f[j] >= bound) visit(rank_key(f[j], at + j));
+    }
+  };
+  const int listed = s_listed;
+  if (listed <= kCand)
+    for (int i = tid; i < listed * vec; i += kThreads)
+      look(list[i / vec], i % vec, [&](unsigned long long key) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kCand) cand[at] = key;
       });
-  for (int i = tid; i < k; i += kThreads) {
-    const unsigned long long key = mine[i];
-    ids[row * k + i] = key == kNone ? -1 : (int32_t)(uint32_t)key;
-    lp[row * k + i] = key == kNone ? -INFINITY : kLn2 * (fmaf(key_value(key), kl, -s_soft[0]) - s_soft[1]);
+  __syncthreads();
+  const auto write = [&](int r, unsigned long long key) {
+    ids[row * k + r] = key == kNone ? -1 : (int32_t)(uint32_t)key;
+    lp[row * k + r] = key == kNone ? -INFINITY : kLn2 * (fmaf(key_value(key), kl, -s_soft[0]) - s_soft[1]);
+  };
+  const int n = s_count;
+  if (max(n, listed) <= kCand) {
+    for (int i = tid; i < n; i += kThreads) {
+      const unsigned long long key = cand[i];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += cand[j] < key;
+      if (r < k) write(r, key);
+    }
+    for (int i = n + tid; i < k; i += kThreads) write(i, kNone);
+    return;
+  }
+  unsigned long long last = 0;                     // below every key of an unmasked logit
+  for (int r = 0; r < k; ++r) {
+    unsigned long long b = kNone;
+    each_top([&](int u, float x) {
+      if (x >= bound)
+        for (int i = 0; i < vec; ++i)
+          look(u << 8 | tid, i, [&](unsigned long long key) {
+            if (key > last && key < b) b = key;
+          });
+    });
+    b = warp_reduce(b, MinKey());
+    __syncthreads();
+    if ((tid & 31) == 0) warp_key[tid >> 5] = b;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) b = min(b, warp_key[w]);
+    if (tid == 0) write(r, b);
+    last = b;
   }
 }
 
@@ -1692,14 +1670,15 @@ struct Carver {
   }
 };
 struct TopWork {
-  unsigned long long *parts, *lists;
+  unsigned long long* parts;
+  float* tops;
   size_t bytes;
 };
-TopWork carve_topk(int64_t units, int k, void* p) {
+TopWork carve_topk(int64_t units, void* p) {
   Carver c{static_cast<char*>(p)};
   TopWork t{};
   t.parts = c.take<unsigned long long>(units);
-  t.lists = c.take<unsigned long long>(units * k);
+  t.tops = c.take<float>(units * kThreads);
   t.bytes = c.used;
   return t;
 }
@@ -1716,40 +1695,35 @@ KdRows carve_kd(int64_t rows, int k, void* p, size_t& bytes) {
 
 }  // namespace
 
-// Vectors per thread and unit of top-k
-static int top_vec(Type type, Logits z, int64_t rows, int V) {
-  return type == F32 && rows * splits_of(type, z, rows, V, 16 * kThreads) >= 2 * sm_count() ? 16 : 8;
-}
-size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V, int k) {
-  return carve_topk(rows * splits_of(type, z, rows, V, top_vec(type, z, rows, V) * kThreads), k, nullptr).bytes;
-}
-cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float temp, int32_t* ids, float* lp,
-                         void* workspace, cudaStream_t stream) {
-  const int vec = top_vec(type, z, rows, V), splits = splits_of(type, z, rows, V, vec * kThreads);
-  const TopWork w = carve_topk(rows * splits, k, workspace);
-  const int groups = k <= 24 ? 32 : k <= 48 ? 64 : k <= 96 ? 128 : 256;
-  Shape units, merge;
-  units.blocks = merge.blocks = rows;
-  units.units = splits;
-  merge.early = true;
-  const cudaError_t e = by_type(type, [&](auto t) {
-    using T = decltype(t);
-    const auto go = [&](auto kernel) {
-      return launch(kernel, units, stream, static_cast<const T*>(z.p), z.ld, rows, V, k, groups, (float)(kLog2ed / temp),
-                    w.parts, w.lists);
-    };
-    if constexpr (sizeof(T) == 4)
-      if (vec == 16) return go(topk_units_kernel<T, 16>);
-    return go(topk_units_kernel<T, 8>);
-  });
-  if (e != cudaSuccess) return e;
-  return launch(topk_merge_kernel, merge, stream, splits, k, groups, (float)(kLog2ed / temp), w.parts, w.lists, ids, lp);
-}
-
-// Vectors per thread and unit of the tail sums
+// Vectors per thread and unit of the sums for top-k and for the loss
 static int part_vec(Type type, Logits z, int64_t rows, int V) {
   return type != F32 && rows * splits_of(type, z, rows, V, 16 * kThreads) >= 2 * sm_count() ? 16 : 8;
 }
+size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V) {
+  return carve_topk(rows * splits_of(type, z, rows, V, part_vec(type, z, rows, V) * kThreads), nullptr).bytes;
+}
+cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float temp, int32_t* ids, float* lp,
+                         void* workspace, cudaStream_t stream) {
+  const int vec = part_vec(type, z, rows, V), splits = splits_of(type, z, rows, V, vec * kThreads);
+  const TopWork w = carve_topk(rows * splits, workspace);
+  const int groups = k <= 24 ? 32 : k <= 48 ? 64 : k <= 96 ? 128 : 256;
+  const float kl = (float)(kLog2ed / temp);
+  Shape units, select;
+  units.blocks = select.blocks = rows;
+  units.units = splits;
+  select.early = true;
+  return by_type(type, [&](auto t) {
+    using T = decltype(t);
+    const T* p = static_cast<const T*>(z.p);
+    const auto go = [&](auto kernel) { return launch(kernel, units, stream, p, z.ld, rows, V, kl, w.parts, w.tops); };
+    cudaError_t e;
+    if constexpr (sizeof(T) == 4) e = go(topk_units_kernel<T, 8>);
+    else e = vec == 16 ? go(topk_units_kernel<T, 16>) : go(topk_units_kernel<T, 8>);
+    if (e != cudaSuccess) return e;
+    return launch(topk_select_kernel<T>, select, stream, p, z.ld, V, vec, splits, k, groups, kl, w.parts, w.tops, ids, lp);
+  });
+}
+
 size_t kd_topk_loss_workspace(Type type, Logits z, int64_t rows, int V) {
   return rows * splits_of(type, z, rows, V, part_vec(type, z, rows, V) * kThreads) * sizeof(unsigned long long);
 }

@@ -68,7 +68,7 @@ void teacher_topk(torch::Tensor logits, double temp, torch::Tensor ids, torch::T
   const float t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(logits.device());
-  const torch::Tensor ws = bytes_like(logits, v::teacher_topk_workspace(type_of(logits), rows_of(logits), n, logits.size(1), k));
+  const torch::Tensor ws = bytes_like(logits, v::teacher_topk_workspace(type_of(logits), rows_of(logits), n, logits.size(1)));
   launched(v::teacher_topk(type_of(logits), rows_of(logits), n, logits.size(1), k, t, ids.data_ptr<int32_t>(),
                            lp.data_ptr<float>(), ws.data_ptr(), at::cuda::getCurrentCUDAStream()),
            "teacher_topk");

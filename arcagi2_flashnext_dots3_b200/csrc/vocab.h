@@ -27,7 +27,7 @@ struct Teacher {                 // [rows, k] ids (int32 or int64) and fp32 log-
 };
 
 // A workspace has the bytes that its ..._workspace() says.
-size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V, int k);
+size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V);
 cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float temp, int32_t* ids, float* lp,
                          void* workspace, cudaStream_t stream);
 
