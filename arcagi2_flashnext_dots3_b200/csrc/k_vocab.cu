@@ -29,13 +29,16 @@
 //   * forms with one look at the logits (top-k, the loss alone, verification) take a unit per block, straight into
 //     registers; a second small kernel, started early, joins the units' parts of a row in order;
 //   * gradients from saved statistics are elementwise: a unit per block;
-//   * forms that look twice (loss with gradient, acceptance) give a row to one block per SM, or to a cluster of them when
-//     there are few rows. A block copies as much of its slice as fits into shared memory (cp.async, read back only by the
-//     thread that copied it) and streams the rest, once for each look: the second time it comes from L2, since 148 such
-//     remainders fit there. Nothing is exchanged outside a cluster, whose blocks write their parts into each other's shared
-//     memory and finish the row's statistics each by itself, in rank order;
+//   * forms that look twice (loss with gradient of more logits than L2 holds, acceptance) give a row to one block, several of
+//     which share an SM, or to a cluster of blocks. A block copies as much of its share as fits into shared memory
+//     (cp.async, read back only by the thread that copied it) and streams the rest, once for each look: the second time it
+//     comes from L2. Nothing is exchanged outside a cluster, whose blocks write their parts into each other's shared
+//     memory and finish the row's statistics each by itself, in rank order. One kernel over both looks without clusters,
+//     its blocks waiting for the other blocks of their row through global memory, took 276 us where this takes 238
+//     (1024 x 151936 fp32), and a loss kernel followed by a gradient kernel 287;
 //   * exp(x) is ex2(x log2 e / T - c) with c = m log2 e / T rounded once and used for the sum and for every
 //     probability alike, so that rounding cancels; one FMA and one ex2 per element.
+// Times below are of one B200, GPU time per call with inputs larger than L2, and "of the copy rate" is of 6551 GB/s.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -54,9 +57,12 @@ constexpr int kBatch = 8;            // vectors that a thread holds at once
 constexpr int kMaxCluster = 16;
 constexpr int kRowThreads = 256;     // of the kernels that look twice
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kRowBlocks = 5;        // their blocks per SM and the vectors of each that shared memory keeps (40 KB):
-constexpr int kRowKeep = 2560;       //   one tensor,
-constexpr int kPairBlocks = 4;       //   two tensors (48 KB; more registers)
+// Their blocks per SM and the vectors of each that shared memory keeps. One tensor: 40 KB in 48 registers (three to six
+// blocks are within 1%). Two tensors: 48 KB and 64 registers; five blocks spill (508 x 151936 bf16: 132 us instead of 118),
+// three are too few to cover the loads (2044 x 32768 fp32: 150 us instead of 136).
+constexpr int kRowBlocks = 5;
+constexpr int kRowKeep = 2560;
+constexpr int kPairBlocks = 4;
 constexpr int kPairKeep = 3072;
 constexpr float kTailFloor = 1e-8f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -515,8 +521,11 @@ __device__ __forceinline__ int load_id(const Teacher& t, int64_t i, int V) {
 // The first kernel reads the logits: softmax parts, and the maximum of each thread's vectors. The second, one block per row,
 // selects: the k-th largest of G >= k group maxima (a group: the logits of kThreads / G threads over all units) is a bound
 // that at least k values reach and few others do (with k = 20 of 32 groups about 31 of independent values). The vectors
-// of threads whose maximum reaches it are read again, one per thread; what reaches it is collected and ranked by counting. More than kCand
-// (long runs of equal logits): k rounds of the smallest key above the last, which any input ends in.
+// of threads whose maximum reaches it are read again, one per thread; what reaches it is collected and ranked by counting.
+// More than kCand (long runs of equal logits): k rounds of the smallest key above the last, which any input ends in.
+// Bound by memory: 105 us for 1024 x 151936 fp32 (91% of the copy rate), 152 us for 2048 x 152064 bf16 (63%: twice the ex2 per
+// byte). Few rows: 12 us for 8 x 151936 fp32, the two kernels' latencies. Selecting in each unit, and joining lists, took
+// 133 and 317 us: the selection's barriers then stand between a block's loads and the next block's.
 constexpr int kCand = 512;
 
 template <typename T, int kVec>
@@ -816,7 +825,8 @@ __device__ __forceinline__ uint4 scaled_exp(const uint4& x, Two scale, Two minus
   return Vec<T>::pack(f);
 }
 
-// The tail's part of one unit: vectors that hold a teacher's token give it up.
+// The tail's part of one unit: vectors that hold a teacher's token give it up. With kd_loss_kernel behind it 92 us for 1024 x
+// 151936 fp32 (103% of the copy rate), 225 us for 4096 x 152064 bf16 (84%), 6.5 us for 16 x 32000 fp32 (latency).
 template <typename T, int kPartVec>
 __global__ void __launch_bounds__(kThreads) kd_parts_kernel(const T* logits, int64_t ld, int64_t rows, int V, Teacher t,
                                                             float kl, unsigned long long* parts) {
@@ -921,7 +931,9 @@ struct ShareIds {
 
 // Loss and gradient of a row by one block or cluster. The owner of a teacher's token takes it out (-inf) before the first
 // look, which so sums the tail alone (a confident student's tail is lost in 1 - sum ps); after the second look it writes
-// the token's gradient.
+// the token's gradient. 238 us for 1024 x 151936 fp32 (80% of the copy rate for one read and one write), 522 us for 4096 x
+// 152064 bf16 (73%). A block's phases (load, reduce, write) leave its share of the memory idle between them, which only the
+// other blocks of the SM fill; in bf16 the two ex2 per 4 bytes take 60% of the time as well.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, kRowBlocks) kd_grad_kernel(const T* logits, int64_t ld, int V, int keep,
                                                                           int k, float kl, float* loss, T* out,
@@ -1028,7 +1040,8 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) kd_grad_kernel(const 
       for (int i = 0; i < 4; ++i) __stcs(p + v + i * kRowThreads, scaled_exp<T>(dyn[v + i * kRowThreads], scale, c2, k2));
   } else {
     for (int v = tid; v < s.n; v += kRowThreads) {
-      const uint4 u = scaled_exp<T>(v < s.kept ? dyn[v] : __ldcg(reinterpret_cast<const uint4*>(s.row + s.e0) + v), scale, c2, k2);
+      const uint4 x = v < s.kept ? dyn[v] : __ldcg(reinterpret_cast<const uint4*>(s.row + s.e0) + v);
+      const uint4 u = scaled_exp<T>(x, scale, c2, k2);
 #pragma unroll
       for (int j = 0; j < N; ++j) o[s.e0 + v * N + j] = reinterpret_cast<const T*>(&u)[j];
     }
@@ -1043,7 +1056,8 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) kd_grad_kernel(const 
     if (s.owns(list.id[j]) || list.id[j] == single) o[list.id[j]] = Vec<T>::back(kd_pull(f, w, list.z[j], list.pt[j], kl));
 }
 
-// The gradient from statistics, elementwise; `out` may be the logits.
+// The gradient from statistics, elementwise; `out` may be the logits. 189 us for 1024 x 151936 fp32, 376 us for 4096 x 152064
+// bf16 (both 101% of the copy rate).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64_t ld, int64_t rows, int V, Teacher t,
                                                           float kl, float inv_t, const float* weight,
@@ -1161,7 +1175,9 @@ __device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&
   a.d += sum(d);
 }
 
-// One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p).
+// One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p). 135 us for 2044 x
+// 32768 fp32 (60% of the copy rate), 118 us for 508 x 151936 bf16 (40%): three ex2 per pair of logits (64 us of the 118) and
+// 33 instructions (70 us at full issue) come near the time of the loads, and the two looks of a block do not overlap.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const T* draft, int64_t ldq, const T* target,
                                                                          int64_t ldp, int V, int keep, float kl, float temp,
@@ -1279,7 +1295,8 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
 
 // Which of q_v, p_v is smaller decides a jump of the gradient, so the comparison is not left to the ex2 arguments, whose
 // rounded offsets are off by up to 2^-20: log-probabilities are formed as a log-softmax forms them, ((z / T) - max) - log
-// sum, each step rounded to fp32. Equal ones take the mean of the two sides.
+// sum, each step rounded to fp32. Equal ones take the mean of the two sides. 117 us for 2044 x 32768 fp32 (105% of the copy
+// rate), 75 us for 508 x 151936 bf16 (94%).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, int64_t ldq, const T* target, int64_t ldp,
                                                               int64_t rows, int V, float kl, float temp,
@@ -1325,10 +1342,13 @@ __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, in
 
 // ------------------------------------------------------------------------------------------- draft verification
 // Two launches. The first reduces every needed row of logits, cut over blocks, to softmax parts (T > 0) or to its best
-// token (T <= 0). The second, several blocks per sequence and started early by programmatic launch, joins the parts,
-// finds the first rejected draft and draws from that position alone: the race costs a hash per token and is run for one row
-// of the k + 1. A draw needs -log(u) / r below the best so far; -log(u) >= 1 - u, which is the hash's integer, so the
-// logarithm and the division are taken for the few tokens that can win.
+// token (T <= 0). The second, as many blocks per sequence as run at once, started early by programmatic launch, joins the
+// parts, finds the first rejected draft and draws from that position alone: the race costs a hash per token and is run for
+// one row of the k + 1. A draw needs -log(u) / r below the best so far; -log(u) >= 1 - u, which is the hash's integer, so
+// the logarithm and the division are taken for the few tokens that can win.
+// 54 us for 64 sequences of 3 soft drafts x 151936 bf16: 30 us the rows (70% of the copy rate), 24 us the draw, bound by the 48
+// instructions per token, most of them the hash's 64-bit products. 34 us for 32 sequences of up to 7 point-mass drafts x
+// 152064 fp32 (70% of the copy rate over both). One sequence of 3: 10 us, latency.
 constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr int kDrawVec = 2;          // vectors that a thread requests at once
@@ -1489,10 +1509,10 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
   const bool same = ((reinterpret_cast<uintptr_t>(qrow) ^ reinterpret_cast<uintptr_t>(row)) & 15) == 0;
   const uint64_t base = seed + (step + acc) * 0xD1B54A32D192ED03ull;
   // The earliest of all times is exponential with the rate sum r: 1 for p, 1 - p(d) beside a point mass. A draw that only
-  // looks for times up to 24 / rate misses them in one of 2^34 cases, and what it saves is the logarithms that each warp
-  // took until it had a bound of its own (39 us to XX us for 64 residuals of 151936 bf16 tokens). The rate of a residual is
-  // not known; 1024 covers all but rates of 1/64 and below, which are rejected as rarely. The block that completes a
-  // sequence without a token repeats the search alone, without the limit, and, if the residual is empty, over p itself.
+  // looks for times up to 24 / rate misses them in one of 2^34 cases, and saves the logarithms that each warp took until it
+  // had a bound of its own. The rate of a residual is not known; 1024 covers all but rates of about 1/64 and below, which
+  // are rejected as rarely. The block that completes a sequence without a token repeats the search alone, without the
+  // limit, and, if the residual is empty, over p itself.
   float limit = 24.f;
   if (qrow) limit = 1024.f;
   else if (id >= 0 && id < a.V) limit = 24.f / fmaxf(1.f - ex2(fmaf(Vec<T>::one(row[id]), kl, -p.c)) * ip, 1e-6f);
@@ -1592,7 +1612,12 @@ int splits_of(Type type, Logits z, int64_t rows, int V, int unit) {
 }
 
 // Blocks per row (a cluster) and vectors of each tensor that a block keeps, in the kernels that look twice; `sides` tensors
-// share a block.
+// share a block. A cluster costs its barriers, so it grows only
+//   * until what all running blocks do not keep takes half of L2, as the second look reads it there (clusters of 1, 2, 4, 8,
+//     16: 1024 x 151936 fp32 with gradient 340, 300, 286, 250, 329 us, taken 8; 2048 x 152064 bf16 312, 283, 271, 353,
+//     547 us, taken 4; acceptance of 2044 x 32768 fp32 159, 136, 167, 240, 479 us, taken 2);
+//   * until one wave of blocks fills the GPU, as long as each thread has a vector (acceptance of 4 x 151936 bf16 46, 27, 18,
+//     13, 11 us, taken 16; 64 x 151936 bf16 51, 30, 23, 23, 31 us, taken 8).
 struct Plan {
   int cluster, keep, smem;
 };
@@ -1695,7 +1720,9 @@ KdRows carve_kd(int64_t rows, int k, void* p, size_t& bytes) {
 
 }  // namespace
 
-// Vectors per thread and unit of the sums for top-k and for the loss
+// Vectors per thread and unit of the sums for top-k and for the loss. 16-bit rows do better with 16 when there are units for
+// every SM (the loss of 2048 x 152064 bf16: 119 us, 124 with 8) and with 8 when there are not (16 x 152064 bf16: 8.8 us, 10.7
+// with 16); fp32 with 8 always (16 x 151936: 8.7 us, 10.3 with 16; 1024 x 151936: 92 us with both).
 static int part_vec(Type type, Logits z, int64_t rows, int V) {
   return type != F32 && rows * splits_of(type, z, rows, V, 16 * kThreads) >= 2 * sm_count() ? 16 : 8;
 }
@@ -1715,7 +1742,9 @@ cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float 
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     const T* p = static_cast<const T*>(z.p);
-    const auto go = [&](auto kernel) { return launch(kernel, units, stream, p, z.ld, rows, V, kl, w.parts, w.tops); };
+    const auto go = [&](auto kernel) {
+      return launch(kernel, units, stream, p, z.ld, rows, V, kl, w.parts, w.tops);
+    };
     cudaError_t e;
     if constexpr (sizeof(T) == 4) e = go(topk_units_kernel<T, 8>);
     else e = vec == 16 ? go(topk_units_kernel<T, 16>) : go(topk_units_kernel<T, 8>);
@@ -1764,10 +1793,12 @@ static cudaError_t kd_from_stats(Type type, Logits z, int64_t rows, int V, Teach
   });
 }
 
-// Logits that fit in L2 are read from there the second time whichever block does it
+// Logits that fit in L2 are read from there the second time whichever block does it, and two grids of units then beat one of
+// clusters (192 x 151936 fp32, 117 MB: 62 us, 74 in clusters; 64 x 152064 bf16: 21 and 26 us); more come from memory again (256
+// x 151936 fp32, 156 MB: 83 us, 77 in clusters).
 static bool kd_in_l2(Type type, int64_t rows, int V) {
   int dev = 0, l2 = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&l2, cudaDevAttrL2CacheSize, dev) != cudaSuccess) return false;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&l2, cudaDevAttrL2CacheSize, dev);
   return rows * V * (type == F32 ? 4 : 2) <= l2;
 }
 size_t kd_topk_grad_workspace(Type type, Logits z, int64_t rows, int V, int k) {
@@ -1797,10 +1828,10 @@ cudaError_t kd_topk_grad(Type type, Logits z, int64_t rows, int V, Teacher t, fl
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     const T* src = static_cast<const T*>(z.p);
-    const cudaError_t e = launch(kd_prepare_kernel<T>, prepare, stream, src, z.ld, V, t, (float)(kLog2ed / temp), 1.f / temp, weight, r);
+    const float kl = (float)(kLog2ed / temp);
+    const cudaError_t e = launch(kd_prepare_kernel<T>, prepare, stream, src, z.ld, V, t, kl, 1.f / temp, weight, r);
     if (e != cudaSuccess) return e;
-    return launch(kd_grad_kernel<T>, grad, stream, src, z.ld, V, p.keep, t.k, (float)(kLog2ed / temp), loss, static_cast<T*>(out),
-                  out_ld, r);
+    return launch(kd_grad_kernel<T>, grad, stream, src, z.ld, V, p.keep, t.k, kl, loss, static_cast<T*>(out), out_ld, r);
   });
 }
 cudaError_t kd_topk_bwd(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, const float* weight,

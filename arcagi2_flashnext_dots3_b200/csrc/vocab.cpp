@@ -107,7 +107,8 @@ void kd_topk_grad(torch::Tensor logits, torch::Tensor t_ids, torch::Tensor t_lp,
   const float t = check_temp(temp);
   if (!n) return;
   const c10::cuda::CUDAGuard guard(logits.device());
-  const torch::Tensor ws = bytes_like(logits, v::kd_topk_grad_workspace(type_of(logits), rows_of(logits), n, logits.size(1), teacher.k));
+  const torch::Tensor ws = bytes_like(
+      logits, v::kd_topk_grad_workspace(type_of(logits), rows_of(logits), n, logits.size(1), teacher.k));
   launched(v::kd_topk_grad(type_of(logits), rows_of(logits), n, logits.size(1), teacher, t, weight.data_ptr<float>(),
                            loss.data_ptr<float>(), out.data_ptr(), out.stride(0), ws.data_ptr(),
                            at::cuda::getCurrentCUDAStream()), "kd_topk_grad");
