@@ -67,16 +67,13 @@ def teacher_topk(logits: torch.Tensor, k: int, temperature: float = 1.0):
     """(ids int32 [rows, k], log-probabilities fp32 [rows, k]) of the k largest logits of each row, best first (ties:
     lowest id), under softmax(logits / temperature). Rows with fewer than k unmasked tokens are padded with id -1 and
     log-probability -inf, the padding of the distillation records. k <= 128."""
+    if logits.is_cuda:
+        return native.C().teacher_topk(logits, k, temperature)
     logits = _rows(logits.detach(), "logits")
     t = _temperature(temperature)
     if not 1 <= k <= MAX_K:
         raise ValueError(f"k must be in [1, {MAX_K}], got {k}")
     n, V = logits.shape
-    if logits.is_cuda:
-        ids = torch.empty(n, k, dtype=torch.int32, device=logits.device)
-        lp = torch.empty(n, k, dtype=torch.float32, device=logits.device)
-        native.C().teacher_topk(logits, t, ids, lp)
-        return ids, lp
     ls = _log_softmax(logits, t)
     z = logits.float()
     order = torch.sort(z.masked_fill(z <= MASKED, float("-inf")), dim=-1, descending=True, stable=True).indices[:, :k]
@@ -114,34 +111,17 @@ def _kd_cpu(logits, t_ids, t_lp, t, weight=None):
     return loss, torch.where(nothing[:, None], 0.0, d).to(logits.dtype)
 
 
-def _kd_loss(logits, t_ids, t_lp, t, stats):
-    if not logits.is_cuda:
-        return _kd_cpu(logits, t_ids, t_lp, t)
-    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-    native.C().kd_topk_loss(logits, t_ids, t_lp, t, loss, stats)
-    return loss
-
-
 class _KDTopK(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, t_ids, t_lp, t):
         ctx.t = t
-        if not logits.is_cuda:
-            ctx.save_for_backward(logits, t_ids, t_lp)
-            return _kd_loss(logits, t_ids, t_lp, t, None)
-        stats = torch.empty(logits.shape[0], native.C().kd_stats, dtype=torch.float32, device=logits.device)
-        ctx.save_for_backward(logits, t_ids, t_lp, stats)
-        return _kd_loss(logits, t_ids, t_lp, t, stats)
+        ctx.save_for_backward(logits, t_ids, t_lp)
+        return _kd_cpu(logits, t_ids, t_lp, t)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        logits, t_ids, t_lp, *stats = ctx.saved_tensors
-        if not logits.is_cuda:
-            return _kd_cpu(logits, t_ids, t_lp, ctx.t, g.float())[1], None, None, None
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        native.C().kd_topk_bwd(logits, t_ids, t_lp, ctx.t, stats[0], g.float().contiguous(), out)
-        return out, None, None, None
+        return _kd_cpu(*ctx.saved_tensors, ctx.t, g.float())[1], None, None, None
 
 
 def kd_topk(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
@@ -149,12 +129,11 @@ def kd_topk(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, tempe
     logits. ``t_ids`` int32 / int64 [rows, K] with K <= 128, ``t_lp`` the teacher's log-probabilities at them (at the
     same temperature). Ids outside the vocabulary (the -1 of padded records) are left out and their mass falls to the
     tail; a repeated id counts once, at its first place. Both tail masses have a floor of 1e-8."""
+    if logits.is_cuda:
+        return native.C().kd_topk(logits, t_ids, t_lp, temperature)
     logits = _rows(logits, "logits")
     t_ids, t_lp = _teacher(logits, t_ids, t_lp)
-    t = _temperature(temperature)
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _KDTopK.apply(logits, t_ids, t_lp, t)
-    return _kd_loss(logits, t_ids, t_lp, t, None)
+    return _KDTopK.apply(logits, t_ids, t_lp, _temperature(temperature))
 
 
 def kd_topk_grad(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, weight: torch.Tensor,
@@ -162,6 +141,8 @@ def kd_topk_grad(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, 
     """(loss [rows], d sum(weight * loss) / d logits in the logits' type) of :func:`kd_topk` in one pass over the
     logits, for callers that know the rows' weights (fp32 [rows]). ``out``: where the gradient goes; it may be the
     logits themselves, which are then overwritten."""
+    if logits.is_cuda:
+        return native.C().kd_topk_grad(logits, t_ids, t_lp, weight, temperature, out)
     logits = _rows(logits.detach(), "logits")
     t_ids, t_lp = _teacher(logits, t_ids, t_lp)
     t = _temperature(temperature)
@@ -174,10 +155,6 @@ def kd_topk_grad(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, 
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or \
             (out.shape[1] > 1 and out.stride(1) != 1):
         raise ValueError("out must have the logits' shape, type and device and unit stride along the vocabulary")
-    if logits.is_cuda:
-        loss = torch.empty(n, dtype=torch.float32, device=logits.device)
-        native.C().kd_topk_grad(logits, t_ids, t_lp, t, weight, loss, out)
-        return loss, out
     loss, g = _kd_cpu(logits, t_ids, t_lp, t, weight)
     return loss, out.copy_(g)
 
@@ -198,36 +175,17 @@ def _accept_cpu(draft, target, t, g_alpha=None, g_kl=None):
     return torch.where(nothing[:, None], 0.0, d).to(draft.dtype)
 
 
-def _accept(draft, target, t, stats):
-    if not draft.is_cuda:
-        return _accept_cpu(draft, target, t)
-    alpha = torch.empty(draft.shape[0], dtype=torch.float32, device=draft.device)
-    kl = torch.empty_like(alpha)
-    native.C().accept_kl(draft, target, t, alpha, kl, stats)
-    return alpha, kl
-
-
 class _AcceptKL(torch.autograd.Function):
     @staticmethod
     def forward(ctx, draft, target, t):
         ctx.t = t
-        if not draft.is_cuda:
-            ctx.save_for_backward(draft, target)
-            return _accept(draft, target, t, None)
-        stats = torch.empty(draft.shape[0], native.C().accept_stats, dtype=torch.float32, device=draft.device)
-        ctx.save_for_backward(draft, target, stats)
-        return _accept(draft, target, t, stats)
+        ctx.save_for_backward(draft, target)
+        return _accept_cpu(draft, target, t)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_alpha, g_kl):
-        draft, target, *stats = ctx.saved_tensors
-        g_alpha, g_kl = g_alpha.float().contiguous(), g_kl.float().contiguous()
-        if not draft.is_cuda:
-            return _accept_cpu(draft, target, ctx.t, g_alpha, g_kl), None, None
-        out = torch.empty(draft.shape, dtype=draft.dtype, device=draft.device)
-        native.C().accept_kl_bwd(draft, target, ctx.t, stats[0], g_alpha, g_kl, out)
-        return out, None, None
+        return _accept_cpu(*ctx.saved_tensors, ctx.t, g_alpha.float(), g_kl.float()), None, None
 
 
 def accept_kl(draft: torch.Tensor, target: torch.Tensor, temperature: float = 1.0):
@@ -235,12 +193,11 @@ def accept_kl(draft: torch.Tensor, target: torch.Tensor, temperature: float = 1.
     min(q_v, p_v), the probability that speculative verification accepts a token drawn from q, and kl = KL(p || q),
     with q, p the softmaxes at `temperature`. Differentiable in the draft; the target is taken as given. Where q_v =
     p_v the gradient of alpha is the mean of its two sides. A row in which either side has no token left gives zeros."""
+    if draft.is_cuda:
+        return native.C().accept_kl(draft, target, temperature)
     draft = _rows(draft, "draft logits")
     target = _rows(target.detach(), "target logits")
     if draft.shape != target.shape or draft.dtype != target.dtype or draft.device != target.device:
         raise ValueError(f"draft and target logits must agree in shape, type and device: {tuple(draft.shape)} "
                          f"{draft.dtype} {draft.device} and {tuple(target.shape)} {target.dtype} {target.device}")
-    t = _temperature(temperature)
-    if draft.requires_grad and torch.is_grad_enabled():
-        return _AcceptKL.apply(draft, target, t)
-    return _accept(draft, target, t, None)
+    return _AcceptKL.apply(draft, target, _temperature(temperature))

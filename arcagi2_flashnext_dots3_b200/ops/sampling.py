@@ -227,6 +227,8 @@ def speculative_verify(logits: torch.Tensor, drafts: torch.Tensor, temps: torch.
     T <= 0 is greedy: accepted while the draft is the argmax (lowest id on ties), which is also the next token. A draft
     outside the vocabulary is rejected. Masked logits (at or below -1e30) are never drawn; a residual that is empty in
     fp32 draws from p; a position with no token left gives -1."""
+    if logits.is_cuda:
+        return native.C().spec_verify(logits, drafts, temps, seeds, steps, draft_logits, n_draft)
     if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
         raise ValueError(f"logits: expected [B, k + 1, V], got {tuple(logits.shape)}")
     B, k1, V = logits.shape
@@ -240,14 +242,6 @@ def speculative_verify(logits: torch.Tensor, drafts: torch.Tensor, temps: torch.
     if draft_logits is not None and (draft_logits.shape != (B, k, V) or draft_logits.dtype != logits.dtype):
         raise ValueError(f"draft_logits: expected {logits.dtype} [{B}, {k}, {V}], got {draft_logits.dtype} "
                          f"{tuple(draft_logits.shape)}")
-    if logits.is_cuda:
-        accepted = torch.empty(B, dtype=torch.int32, device=logits.device)
-        nxt = torch.empty_like(accepted)
-        unit = lambda x: x if x is None or V == 1 or x.stride(2) == 1 else x.contiguous()  # noqa: E731
-        native.C().spec_verify(unit(logits.detach()), drafts.contiguous(), temps.contiguous(), seeds.contiguous(),
-                               steps.contiguous(), unit(draft_logits), None if n_draft is None else n_draft.contiguous(),
-                               accepted, nxt)
-        return accepted, nxt
     got = [_verify_one(logits[b], drafts[b].tolist()[:k if n_draft is None else max(0, int(n_draft[b]))],
                        float(temps[b]), int(seeds[b]), int(steps[b]),
                        None if draft_logits is None else draft_logits[b]) for b in range(B)]

@@ -134,3 +134,39 @@ def test_top_tokens_among_many_equal_logits(dtype):
             assert ids[2].tolist() == list(range(1, 2 * k, 2))
             want = torch.log_softmax(x.double(), -1).gather(1, ids.long())
             assert float((lp.double() - want).abs().max()) <= TOL
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_autograd_edges(device):
+    """Strided logits, an unused output, mixed precision of the incoming gradient, no graph under no_grad, and an error in
+    place of a second derivative."""
+    g = torch.Generator().manual_seed(8)
+    base = torch.randn(40, 6, generator=g).to(device).requires_grad_()
+    x = base.t()                                                         # [6, 40], not unit stride
+    ids = torch.randint(0, 40, (6, 4), generator=g).to(device)
+    lp = torch.log_softmax(torch.randn(6, 5, generator=g), -1)[:, :4].to(device)
+    y = torch.randn(6, 40, generator=g).to(device)
+    _, want = distill.kd_topk_grad(x, ids, lp, torch.ones(6, device=device))
+    got, = torch.autograd.grad(distill.kd_topk(x, ids, lp).sum(), base)
+    assert float((got.t() - want).abs().max()) <= 1e-6
+    both, = torch.autograd.grad(sum(t.sum() for t in distill.accept_kl(x, y)), base)
+    one, = torch.autograd.grad(distill.accept_kl(x, y)[0].sum(), base)
+    other, = torch.autograd.grad(distill.accept_kl(x, y)[1].sum(), base)
+    assert float((both - one - other).abs().max()) <= 1e-6
+    h = x.detach().to(torch.bfloat16).requires_grad_()
+    (distill.kd_topk(h, ids, lp).double() * 2).sum().backward()
+    assert h.grad.dtype == torch.bfloat16 and bool(torch.isfinite(h.grad).all())
+    with torch.no_grad():
+        assert not distill.kd_topk(x, ids, lp).requires_grad and not distill.accept_kl(x, y)[0].requires_grad
+    assert not distill.kd_topk(x.detach(), ids, lp).requires_grad
+    for loss in (distill.kd_topk(x, ids, lp).sum(), distill.accept_kl(x, y)[1].sum()):
+        d, = torch.autograd.grad(loss, base, create_graph=True)
+        with pytest.raises(RuntimeError):
+            d.square().sum().backward()
+    z = y.clone().requires_grad_()
+    t = z * 1.0
+    loss = distill.accept_kl(t, y)[1].sum()
+    with torch.no_grad():
+        t.add_(1.0)                                                      # what backward reads was overwritten
+    with pytest.raises(RuntimeError):
+        loss.backward()
