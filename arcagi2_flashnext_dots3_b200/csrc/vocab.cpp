@@ -174,6 +174,7 @@ std::tuple<torch::Tensor, torch::Tensor> kd_topk_grad(torch::Tensor logits, torc
   launched(v::kd_topk_grad(type_of(logits), rows_of(logits), n, V, teacher, t, weight.data_ptr<float>(),
                            loss.data_ptr<float>(), out.data_ptr(), out.stride(0), ws.data_ptr(),
                            at::cuda::getCurrentCUDAStream()), "kd_topk_grad");
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();    // what was saved of it is gone
   return {loss, out};
 }
 

@@ -20,7 +20,7 @@ import torch
 
 from . import native
 
-MASKED = -1e30       # csrc/k_vocab.cu kMasked
+MASKED = -1e30       # csrc/k_vocab.cu kFloor is the float above it
 TAIL_FLOOR = 1e-8    # csrc/k_vocab.cu kTailFloor
 MAX_K = 128          # csrc/vocab.h kMaxK
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)

@@ -170,3 +170,18 @@ def test_autograd_edges(device):
         t.add_(1.0)                                                      # what backward reads was overwritten
     with pytest.raises(RuntimeError):
         loss.backward()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_gradient_written_over_saved_logits_is_noticed(device):
+    """kd_topk_grad over logits that another function has saved for its backward: that backward raises."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(3, 50, generator=g).to(device).requires_grad_()
+    z = x * 2.0
+    ids = torch.randint(0, 50, (3, 4), generator=g).to(device)
+    lp = torch.full((3, 4), -2.0, device=device)
+    loss = distill.accept_kl(z, z.detach().flip(0))[0].sum()
+    with torch.no_grad():
+        distill.kd_topk_grad(z, ids, lp, torch.ones(3, device=device), out=z.detach())
+    with pytest.raises(RuntimeError):
+        loss.backward()
