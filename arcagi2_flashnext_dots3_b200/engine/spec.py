@@ -152,6 +152,7 @@ class SpecGraph:
             drafts = self.ids[:, 1:].contiguous()
             acc, nxt = sampling.speculative_verify(m.logits(x).view(B, k1, -1), drafts, self.temps, self.seeds, self.steps)
             at = torch.arange(k1, device=x.device)[None]
+            # y[j] is draft j while it was accepted, then the drawn token (0 where nothing could be drawn: no logit left)
             y = torch.where(at < acc[:, None], torch.cat([drafts, nxt[:, None]], 1),
                             torch.where(at == acc[:, None], nxt[:, None], 0)).clamp_min(0)
         else:
@@ -304,7 +305,7 @@ class SpecDecoder:
             t = [torch.tensor(v, dtype=ty).to(lg.device) for v, ty in
                  ((temps, torch.float32), (seeds, torch.int64), (steps, torch.int64))]
             acc, nxt = sampling.speculative_verify(lg, dr.to(lg.device), *t)
-            return acc.tolist(), nxt.clamp_min(0).tolist()
+            return acc.tolist(), nxt.clamp_min(0).tolist()         # -1: no logit left to draw
         return sampling.speculative_accept(lg.float(), dr, temps, seeds, steps)
 
     def _advance(self, seqs, drafts, y, accepted) -> dict:
