@@ -53,7 +53,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBatch = 8;            // vectors that a thread holds at once
+// Vectors per thread and unit. 16 gained the loss 2% above 1000 rows of 16-bit logits and lost 7% at 333 x 151935; top-k lost
+// 10% everywhere, and fp32 never gained.
+constexpr int kUnit = 8;
 constexpr int kMaxCluster = 16;
 constexpr int kRowThreads = 256;     // of the kernels that look twice
 constexpr int kRowWarps = kRowThreads / 32;
@@ -241,9 +243,9 @@ __device__ __forceinline__ uint4 ragged_vec(const Slice<T>& s, const T* row, int
   return Vec<T>::pack(f);
 }
 template <typename T, int kVec>
-__device__ __forceinline__ void load_unit(const Slice<T>& s, const T* row, int first, uint4 (&x)[kVec]) {
+__device__ __forceinline__ void load_unit(const Slice<T>& s, const T* row, uint4 (&x)[kVec]) {
   const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(s.row)) & 15) == 0;
-  const int v = first + threadIdx.x;
+  const int v = threadIdx.x;
   if (same && s.inside) {
     const uint4* p = reinterpret_cast<const uint4*>(row + s.start(v));
 #pragma unroll
@@ -258,7 +260,7 @@ __device__ __forceinline__ void load_unit(const Slice<T>& s, const T* row, int f
 }
 template <typename T, int kVec>
 __device__ __forceinline__ void load_unit(const Slice<T>& s, uint4 (&x)[kVec]) {
-  load_unit(s, s.row, 0, x);
+  load_unit(s, s.row, x);
 }
 // A block's share of a row in the kernels that look twice: `n` whole vectors from element `e0`, which lies on a 16-byte
 // boundary, and the elements in front of the row's first boundary and behind its last, which the first and the last block
@@ -523,12 +525,12 @@ __device__ __forceinline__ int load_id(const Teacher& t, int64_t i, int V) {
 // that at least k values reach and few others do (with k = 20 of 32 groups about 31 of independent values). The vectors
 // of threads whose maximum reaches it are read again, one per thread; what reaches it is collected and ranked by counting.
 // More than kCand (long runs of equal logits): k rounds of the smallest key above the last, which any input ends in.
-// Bound by memory: 105 us for 1024 x 151936 fp32 (91% of the copy rate), 152 us for 2048 x 152064 bf16 (63%: twice the ex2 per
+// Bound by memory: 103 us for 1024 x 151936 fp32 (93% of the copy rate), 138 us for 2048 x 152064 bf16 (69%: twice the ex2 per
 // byte). Few rows: 12 us for 8 x 151936 fp32, the two kernels' latencies. Selecting in each unit, and joining lists, took
 // 133 and 317 us: the selection's barriers then stand between a block's loads and the next block's.
 constexpr int kCand = 512;
 
-template <typename T, int kVec>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, int64_t ld, int64_t rows, int V, float kl,
                                                               unsigned long long* parts, float* tops) {
   __shared__ unsigned long long warp_part[kWarps];
@@ -536,16 +538,12 @@ __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, i
   pdl_launch_dependents();
   const int64_t row = unit_row();
   if (row >= rows) return;
-  const Slice<T> s(logits + row * ld, V, kVec * kThreads, blockIdx.x);
-  float m = kFloor, top = -INFINITY;
+  const Slice<T> s(logits + row * ld, V, kUnit * kThreads, blockIdx.x);
+  float m = kFloor;
   Soft soft{kFloor * kl, 0.f};
-#pragma unroll
-  for (int b = 0; b < kVec / kBatch; ++b) {
-    uint4 x[kBatch];
-    load_unit(s, s.row, b * kBatch * kThreads, x);
-    top = fmaxf(top, add_soft<T>(x, kl, m, soft));
-  }
-  tops[unit_index() * kThreads + tid] = top;
+  uint4 x[kUnit];
+  load_unit(s, x);
+  tops[unit_index() * kThreads + tid] = add_soft<T>(x, kl, m, soft);
 #pragma unroll
   for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
   if ((tid & 31) == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
@@ -556,9 +554,8 @@ __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, i
   }
 }
 
-// `vec`: vectors per thread and unit of the first kernel
 template <typename T>
-__global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, int64_t ld, int V, int vec, int units, int k,
+__global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, int64_t ld, int V, int units, int k,
                                                                int groups, float kl, const unsigned long long* parts,
                                                                const float* tops, int32_t* ids, float* lp) {
   constexpr int N = Vec<T>::N;
@@ -611,7 +608,7 @@ __global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, 
   __syncthreads();
   // visits the logits that reach the bound in vector i of the thread and unit `from`
   const auto look = [&](int from, int i, auto visit) {
-    const int at = s.start(((from >> 8) * vec + i) * kThreads + (from & 255));
+    const int at = s.start(((from >> 8) * kUnit + i) * kThreads + (from & 255));
     const uint4 x = s.full(at) ? __ldcg(reinterpret_cast<const uint4*>(s.row + at)) : ragged_vec(s, s.row, at);
     if (packed_max<T>(x) >= bound) {
       float f[N];
@@ -623,8 +620,8 @@ __global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, 
   };
   const int listed = s_listed;
   if (listed <= kCand)
-    for (int i = tid; i < listed * vec; i += kThreads)
-      look(list[i / vec], i % vec, [&](unsigned long long key) {
+    for (int i = tid; i < listed * kUnit; i += kThreads)
+      look(list[i / kUnit], i % kUnit, [&](unsigned long long key) {
         const int at = atomicAdd(&s_count, 1);
         if (at < kCand) cand[at] = key;
       });
@@ -649,7 +646,7 @@ __global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, 
     unsigned long long b = kNone;
     each_top([&](int u, float x) {
       if (x >= bound)
-        for (int i = 0; i < vec; ++i)
+        for (int i = 0; i < kUnit; ++i)
           look(u << 8 | tid, i, [&](unsigned long long key) {
             if (key > last && key < b) b = key;
           });
@@ -677,7 +674,6 @@ __device__ __forceinline__ bool repeats(const int* ids, int i) {
   return r;
 }
 
-constexpr int kKdVec = 8;            // vectors per thread and unit of the gradient from statistics
 constexpr int kE = kMaxK / 32;       // teacher entries per lane: entry lane + 32 i
 
 // Lists the places in a slice of the tokens id[0 .. kE) over one warp; returns their number.
@@ -826,8 +822,8 @@ __device__ __forceinline__ uint4 scaled_exp(const uint4& x, Two scale, Two minus
 }
 
 // The tail's part of one unit: vectors that hold a teacher's token give it up. With kd_loss_kernel behind it 92 us for 1024 x
-// 151936 fp32 (103% of the copy rate), 225 us for 4096 x 152064 bf16 (84%), 6.5 us for 16 x 32000 fp32 (latency).
-template <typename T, int kPartVec>
+// 151936 fp32 (103% of the copy rate), 236 us for 4096 x 152064 bf16 (80%), 6.5 us for 16 x 32000 fp32 (latency).
+template <typename T>
 __global__ void __launch_bounds__(kThreads) kd_parts_kernel(const T* logits, int64_t ld, int64_t rows, int V, Teacher t,
                                                             float kl, unsigned long long* parts) {
   constexpr int N = Vec<T>::N;
@@ -837,8 +833,8 @@ __global__ void __launch_bounds__(kThreads) kd_parts_kernel(const T* logits, int
   pdl_launch_dependents();
   const int64_t row = unit_row();
   if (row >= rows) return;
-  const Slice<T> s(logits + row * ld, V, kPartVec * kThreads, blockIdx.x);
-  uint4 x[kBatch];
+  const Slice<T> s(logits + row * ld, V, kUnit * kThreads, blockIdx.x);
+  uint4 x[kUnit];
   load_unit(s, x);
   if (tid < 32) {
     int id[kE];
@@ -850,18 +846,14 @@ __global__ void __launch_bounds__(kThreads) kd_parts_kernel(const T* logits, int
   const int listed = s_listed;
   float m = kFloor;
   Soft soft{kFloor * kl, 0.f};
+  for (int j = 0; j < listed; ++j) {
+    const int v = places[j] / N;
+    if (v % kThreads == tid)
 #pragma unroll
-  for (int b = 0; b < kPartVec / kBatch; ++b) {
-    if (b) load_unit(s, s.row, b * kBatch * kThreads, x);
-    for (int j = 0; j < listed; ++j) {
-      const int v = places[j] / N - b * kBatch * kThreads;
-      if (v % kThreads == tid)
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-          if (v == tid + i * kThreads) x[i] = without<T>(x[i], places[j] % N);
-    }
-    add_soft<T>(x, kl, m, soft);
+      for (int i = 0; i < kUnit; ++i)
+        if (v == tid + i * kThreads) x[i] = without<T>(x[i], places[j] % N);
   }
+  add_soft<T>(x, kl, m, soft);
 #pragma unroll
   for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
   if ((tid & 31) == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
@@ -1064,8 +1056,8 @@ __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64
                                                           const KdRow* stats, T* out, int64_t out_ld) {
   const int64_t row = unit_row();
   if (row >= rows) return;
-  const Slice<T> s(logits + row * ld, V, kKdVec * kThreads, blockIdx.x);
-  uint4 x[kKdVec];
+  const Slice<T> s(logits + row * ld, V, kUnit * kThreads, blockIdx.x);
+  uint4 x[kUnit];
   load_unit(s, x);
   T* o = out + row * out_ld;
   const int tid = threadIdx.x;
@@ -1077,7 +1069,7 @@ __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64
   const float w = st.inv_s == 0.f ? 0.f : weight[row] * inv_t;
   const Two scale = two(st.inv_s == 0.f ? 0.f : -st.csum * st.inv_s * w), c2 = two(-st.c), k2 = two(kl);
   __syncthreads();                                     // every z is read
-  store_unit<kKdVec>(s, o, [&](int i) { return scaled_exp<T>(x[i], scale, c2, k2); });
+  store_unit<kUnit>(s, o, [&](int i) { return scaled_exp<T>(x[i], scale, c2, k2); });
   __syncthreads();
   if (id >= 0) {
     bool repeated = false;
@@ -1308,7 +1300,7 @@ __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, in
   const Slice<T> s(draft + row * ldq, V, kPairVec * kThreads, blockIdx.x);
   uint4 xq[kPairVec], xp[kPairVec];
   load_unit(s, xq);
-  load_unit(s, target + row * ldp, 0, xp);
+  load_unit(s, target + row * ldp, xp);
   const AcceptRow st = stats[row];
   const bool nothing = st.fq == 0.f;
   const float ga = g_alpha[row] / temp, gk = g_kl[row] / temp;
@@ -1403,8 +1395,8 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
   if ((draft ? j - a.k - 1 >= n : j > n) || (draft && greedy)) return;
   const T* row = draft ? static_cast<const T*>(a.draft_logits) + b * a.draft_b + (j - a.k - 1) * a.draft_j
                        : static_cast<const T*>(a.logits) + b * a.logits_b + j * a.logits_j;
-  const Slice<T> s(row, a.V, kBatch * kThreads, split);
-  uint4 x[kBatch];
+  const Slice<T> s(row, a.V, kUnit * kThreads, split);
+  uint4 x[kUnit];
   load_unit(s, x);
   const float top = unit_max<T>(x);
   unsigned long long res;
@@ -1413,7 +1405,7 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
     const float best = warp_reduce(top, Max());
     if (top == best && best >= kFloor) {
 #pragma unroll
-      for (int i = kBatch - 1; i >= 0; --i) {          // ends at the thread's first element of that value
+      for (int i = kUnit - 1; i >= 0; --i) {          // ends at the thread's first element of that value
         float f[N];
         Vec<T>::unpack(x[i], f);
 #pragma unroll
@@ -1605,10 +1597,10 @@ int sm_count() {
 }
 
 // Units per row of `z`: a row that starts off a 16-byte boundary may touch one vector more.
-int splits_of(Type type, Logits z, int64_t rows, int V, int unit) {
+int splits_of(Type type, Logits z, int64_t rows, int V, int vec = kUnit) {
   const int lanes = type == F32 ? 4 : 8;
   const bool aligned = (reinterpret_cast<uintptr_t>(z.p) & 15) == 0 && (rows == 1 || z.ld % lanes == 0);
-  return ((V + lanes - 1) / lanes + (aligned ? 0 : 1) + unit - 1) / unit;
+  return ((V + lanes - 1) / lanes + (aligned ? 0 : 1) + vec * kThreads - 1) / (vec * kThreads);
 }
 
 // Blocks per row (a cluster) and vectors of each tensor that a block keeps, in the kernels that look twice; `sides` tensors
@@ -1720,18 +1712,12 @@ KdRows carve_kd(int64_t rows, int k, void* p, size_t& bytes) {
 
 }  // namespace
 
-// Vectors per thread and unit of the sums for top-k and for the loss. 16-bit rows do better with 16 when there are units for
-// every SM (the loss of 2048 x 152064 bf16: 119 us, 124 with 8) and with 8 when there are not (16 x 152064 bf16: 8.8 us, 10.7
-// with 16); fp32 with 8 always (16 x 151936: 8.7 us, 10.3 with 16; 1024 x 151936: 92 us with both).
-static int part_vec(Type type, Logits z, int64_t rows, int V) {
-  return type != F32 && rows * splits_of(type, z, rows, V, 16 * kThreads) >= 2 * sm_count() ? 16 : 8;
-}
 size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V) {
-  return carve_topk(rows * splits_of(type, z, rows, V, part_vec(type, z, rows, V) * kThreads), nullptr).bytes;
+  return carve_topk(rows * splits_of(type, z, rows, V), nullptr).bytes;
 }
 cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float temp, int32_t* ids, float* lp,
                          void* workspace, cudaStream_t stream) {
-  const int vec = part_vec(type, z, rows, V), splits = splits_of(type, z, rows, V, vec * kThreads);
+  const int splits = splits_of(type, z, rows, V);
   const TopWork w = carve_topk(rows * splits, workspace);
   const int groups = k <= 24 ? 32 : k <= 48 ? 64 : k <= 96 ? 128 : 256;
   const float kl = (float)(kLog2ed / temp);
@@ -1742,23 +1728,18 @@ cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float 
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     const T* p = static_cast<const T*>(z.p);
-    const auto go = [&](auto kernel) {
-      return launch(kernel, units, stream, p, z.ld, rows, V, kl, w.parts, w.tops);
-    };
-    cudaError_t e;
-    if constexpr (sizeof(T) == 4) e = go(topk_units_kernel<T, 8>);
-    else e = vec == 16 ? go(topk_units_kernel<T, 16>) : go(topk_units_kernel<T, 8>);
+    const cudaError_t e = launch(topk_units_kernel<T>, units, stream, p, z.ld, rows, V, kl, w.parts, w.tops);
     if (e != cudaSuccess) return e;
-    return launch(topk_select_kernel<T>, select, stream, p, z.ld, V, vec, splits, k, groups, kl, w.parts, w.tops, ids, lp);
+    return launch(topk_select_kernel<T>, select, stream, p, z.ld, V, splits, k, groups, kl, w.parts, w.tops, ids, lp);
   });
 }
 
 size_t kd_topk_loss_workspace(Type type, Logits z, int64_t rows, int V) {
-  return rows * splits_of(type, z, rows, V, part_vec(type, z, rows, V) * kThreads) * sizeof(unsigned long long);
+  return rows * splits_of(type, z, rows, V) * sizeof(unsigned long long);
 }
 cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, float temp, float* loss, float* stats,
                          void* workspace, cudaStream_t stream) {
-  const int vec = part_vec(type, z, rows, V), splits = splits_of(type, z, rows, V, vec * kThreads);
+  const int splits = splits_of(type, z, rows, V);
   unsigned long long* words = static_cast<unsigned long long*>(workspace);
   Shape parts, last;
   parts.blocks = last.blocks = rows;
@@ -1768,12 +1749,7 @@ cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, fl
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     const T* p = static_cast<const T*>(z.p);
-    const auto go = [&](auto kernel) {
-      return launch(kernel, parts, stream, p, z.ld, rows, V, t, (float)(kLog2ed / temp), words);
-    };
-    cudaError_t e;
-    if constexpr (sizeof(T) == 4) e = go(kd_parts_kernel<T, 8>);
-    else e = vec == 16 ? go(kd_parts_kernel<T, 16>) : go(kd_parts_kernel<T, 8>);
+    const cudaError_t e = launch(kd_parts_kernel<T>, parts, stream, p, z.ld, rows, V, t, (float)(kLog2ed / temp), words);
     if (e != cudaSuccess) return e;
     return launch(kd_loss_kernel<T>, last, stream, p, z.ld, splits, V, t, (float)(kLog2ed / temp), words, loss,
                   reinterpret_cast<KdRow*>(stats));
@@ -1784,7 +1760,7 @@ static cudaError_t kd_from_stats(Type type, Logits z, int64_t rows, int V, Teach
                                  const float* stats, void* out, int64_t out_ld, bool early, cudaStream_t stream) {
   Shape s;
   s.blocks = rows;
-  s.units = splits_of(type, z, rows, V, kKdVec * kThreads);
+  s.units = splits_of(type, z, rows, V);
   s.early = early;
   return by_type(type, [&](auto x) {
     using T = decltype(x);
@@ -1857,7 +1833,7 @@ cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, 
                           const float* g_alpha, const float* g_kl, void* out, int64_t out_ld, cudaStream_t stream) {
   Shape s;
   s.blocks = rows;
-  s.units = splits_of(type, draft, rows, V, kPairVec * kThreads);
+  s.units = splits_of(type, draft, rows, V, kPairVec);
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     return launch(accept_bwd_kernel<T>, s, stream, static_cast<const T*>(draft.p), draft.ld,
@@ -1872,7 +1848,7 @@ struct VerifyPlan {
 };
 VerifyPlan verify_plan(const Verify& a) {
   const int lanes = a.type == F32 ? 4 : 8, total = (a.V + lanes - 1) / lanes + 1;
-  return {(total + kBatch * kThreads - 1) / (kBatch * kThreads), a.draft_logits ? 2 * a.k + 1 : a.k + 1};
+  return {(total + kUnit * kThreads - 1) / (kUnit * kThreads), a.draft_logits ? 2 * a.k + 1 : a.k + 1};
 }
 }  // namespace
 
