@@ -1079,11 +1079,10 @@ __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64
 }
 
 // ------------------------------------------------------------------------------------------- acceptance and KL
-// log2 q_v = zq_v kl - bq up to the rounding of bq, whose remainder is in fq = 2^(rounded - exact), and for p alike; a =
-// sum_v q_v h_v. fq = 0 marks a row with nothing to compare. mq, lq, mp, lp: maxima (divided by T) and log-sums, from which
-// the gradient forms the log-probabilities that it compares.
+// log2 q_v = zq_v kl - bq up to the rounding of bq, whose remainder is in fq = 2^(rounded - exact), and for p alike. fq = 0 marks
+// a row with nothing to compare. steep, middle: h_v = (zq_v - zp_v) steep + middle, held to [0, 1] (share2); a = sum_v q_v h_v.
 struct AcceptRow {
-  float bq, fq, bp, fp, a, mq, lq, mp, lp;
+  float bq, fq, bp, fp, steep, middle, a;
 };
 static_assert(sizeof(AcceptRow) == kAcceptStats * 4, "AcceptRow is what callers allocate");
 
@@ -1101,8 +1100,8 @@ __device__ __forceinline__ Pair join(const Pair& a, const Pair& b, float kl) {
   const float cq = offset(r.mq, kl), cp = offset(r.mp, kl);
   const float qa = offset(a.mq, kl) - cq, qb = offset(b.mq, kl) - cq, pa = offset(a.mp, kl) - cp, pb = offset(b.mp, kl) - cp;
   const float ea = ex2(pa), eb = ex2(pb);
-  r.sq = a.sq * ex2(qa) + b.sq * ex2(qb);
-  r.sp = a.sp * ea + b.sp * eb;
+  r.sq = fmaf(a.sq, ex2(qa), __fmul_rn(b.sq, ex2(qb)));    // one order for both: equal sides stay equal to the last bit
+  r.sp = fmaf(a.sp, ea, __fmul_rn(b.sp, eb));
   // the arguments move by the change of their offsets; a part whose weight vanishes adds nothing, even if infinite
   const float da = a.d + a.sp * (pa - qa), db = b.d + b.sp * (pb - qb);
   r.d = (ea == 0.f ? 0.f : ea * da) + (eb == 0.f ? 0.f : eb * db);
@@ -1114,6 +1113,17 @@ __device__ __forceinline__ Pair shfl_xor(const Pair& a, int o) {
 }
 
 constexpr int kPairVec = 4;          // vectors per thread, unit and side of the gradient
+
+// h of two tokens: 1 where q < p, 0 where q > p, 1/2 where they are equal. With gap the log2 of the ratio of the sums, log2 q_v -
+// log2 p_v = (zq_v - zp_v) kl - gap; the difference of the logits comes first and keeps the digits that the ex2 arguments
+// lose to their offsets. Sums that differ by less than 2^-21 of themselves, a few roundings, count as equal, and within 2^-21 (1
+// + |gap|) of equality, what gap itself may be off by, h goes from 1 to 0 in a line. A = sum q h must take each token's h as the
+// token itself does, or a sure token gets a gradient of full size where 1 - q is all there is: so the forward and the backward
+// form h by these operations alone. One FMA and one saturating FMA; a NaN (both masked by -inf) becomes 0, for tokens without mass.
+__device__ __forceinline__ float2 share2(Two q, Two p, float steep, float middle) {
+  const float2 d = halves(fma2(p, two(-1.f), q));
+  return {__saturatef(fmaf(d.x, steep, middle)), __saturatef(fmaf(d.y, steep, middle))};
+}
 
 template <typename Load>
 __device__ __forceinline__ Pair join_pairs(int n, float kl, Load load) {
@@ -1167,12 +1177,13 @@ __device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&
   a.d += sum(d);
 }
 
-// One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p). 135 us for 2044 x
-// 32768 fp32 (60% of the copy rate), 118 us for 508 x 151936 bf16 (40%): three ex2 per pair of logits (64 us of the 118) and
-// 33 instructions (70 us at full issue) come near the time of the loads, and the two looks of a block do not overlap.
+// One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p) and of q h. 138 us for 2044
+// x 32768 fp32 (59% of the copy rate), 122 us for 508 x 151936 bf16 (39%): three ex2 per pair of logits (64 us of the 122) and
+// some 34 instructions come near the time of the loads, and the two looks of a block do not overlap. h by comparisons, with the
+// few equal tokens in a branch, took 143 and 129 us; with the mass of q on either side summed by itself (a fourth ex2) 144 and 133.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const T* draft, int64_t ldq, const T* target,
-                                                                         int64_t ldp, int V, int keep, float kl, float temp,
+                                                                         int64_t ldp, int V, int keep, float kl,
                                                                          float* alpha, float* out_kl, AcceptRow* stats) {
   constexpr int N = Vec<T>::N;
   extern __shared__ uint4 dyn[];
@@ -1228,7 +1239,10 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
     return Pair{q.c, q.sum, p.c, p.sum, as_soft(part[2][i]).c};
   });
   const float cq = offset(a.mq, kl), cp = offset(a.mp, kl), rq = cq + log2f(a.sq), rp = cp + log2f(a.sp);
-  float under = 0.f, over = 0.f;             // sums of min(q, p) where q <= p and where q > p
+  const float ratio = log2f(__fdiv_rn(a.sq, a.sp)), gap = (cq - cp) + (fabsf(ratio) < 0x1p-21f ? 0.f : ratio);
+  const float per_tie = 0x1p20f / (1.f + fabsf(gap));
+  const float steep = -kl * per_tie, middle = fmaf(gap, per_tie, 0.5f);
+  Two least = two(0.f), held = two(0.f);     // sums of min(q, p), and of it times h: sum q h, as h = 0 where q > p
   const Two k2 = two(kl), bq = two(-rq), bp = two(-rp);
   const auto look = [&](const uint4& uq, const uint4& up) {
     float q[N], p[N];
@@ -1236,12 +1250,11 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
     Vec<T>::unpack(up, p);
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
-      const float2 eq = halves(fma2(two(q[k], q[k + 1]), k2, bq)), ep = halves(fma2(two(p[k], p[k + 1]), k2, bp));
-      const float e0 = ex2(fminf(eq.x, ep.x)), e1 = ex2(fminf(eq.y, ep.y));
-      if (eq.x <= ep.x) under += e0;
-      else over += e0;
-      if (eq.y <= ep.y) under += e1;
-      else over += e1;
+      const Two zq = two(q[k], q[k + 1]), zp = two(p[k], p[k + 1]);
+      const float2 eq = halves(fma2(zq, k2, bq)), ep = halves(fma2(zp, k2, bp)), h = share2(zq, zp, steep, middle);
+      const Two e = two(ex2(fminf(eq.x, ep.x)), ex2(fminf(eq.y, ep.y)));
+      least = add2(least, e);
+      held = fma2(e, two(h.x, h.y), held);
     }
   };
   for (int v = s.kept + tid; v < s.n; v += 2 * kRowThreads) {
@@ -1254,9 +1267,8 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
   if (single >= 0) look(lone[0][0], lone[1][0]);
 #pragma unroll 2
   for (int v = tid; v < s.kept; v += kRowThreads) look(dq[v], dp[v]);
-  under = warp_reduce(under, Add());
-  over = warp_reduce(over, Add());
-  if (lane == 0) warp_sum[tid >> 5] = make_float2(under, over);
+  const float x = warp_reduce(sum(least), Add()), y = warp_reduce(sum(held), Add());
+  if (lane == 0) warp_sum[tid >> 5] = make_float2(x, y);
   __syncthreads();
   if (tid < 32) {
     float2 w = lane < kRowWarps ? warp_sum[lane] : make_float2(0.f, 0.f);
@@ -1266,32 +1278,26 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
   }
   cluster_sync();
   if (rank != 0 || tid != 0) return;
-  float x = 0.f, y = 0.f;
+  float2 w = make_float2(0.f, 0.f);
   for (uint32_t i = 0; i < size; ++i) {
-    x += as_soft(sums[i]).c;
-    y += as_soft(sums[i]).sum;
+    w.x += as_soft(sums[i]).c;
+    w.y += as_soft(sums[i]).sum;
   }
   const double lq = log2((double)a.sq), lp = log2((double)a.sp);
   const float fq = exp2f((float)((double)rq - (cq + lq))), fp = exp2f((float)((double)rp - (cp + lp)));
   const bool nothing = a.sq == 0.f || a.sp == 0.f;
   const bool nan = isnan(a.sq) || isnan(a.sp);            // the minimum drops a NaN operand
-  alpha[row] = nothing ? 0.f : nan ? NAN : fq * x + fp * y;
+  alpha[row] = nothing ? 0.f : nan ? NAN : fp * w.x + (fq - fp) * w.y;
   out_kl[row] = nothing ? 0.f : (float)(kLn2d * ((double)a.d / a.sp + lq - lp));
   if (!stats) return;
-  const float mq = a.mq / temp, mp = a.mp / temp;
-  // natural log of sum exp((z - m) / T): the offsets' roundings taken back
-  const float log_q = (float)(kLn2d * (lq + ((double)cq - (double)a.mq * kl)));
-  const float log_p = (float)(kLn2d * (lp + ((double)cp - (double)a.mp * kl)));
-  stats[row] = nothing ? AcceptRow{} : AcceptRow{rq, fq, rp, fp, fq * x, mq, log_q, mp, log_p};
+  stats[row] = nothing ? AcceptRow{} : AcceptRow{rq, fq, rp, fp, steep, middle, fq * w.y};
 }
 
-// Which of q_v, p_v is smaller decides a jump of the gradient, so the comparison is not left to the ex2 arguments, whose
-// rounded offsets are off by up to 2^-20: log-probabilities are formed as a log-softmax forms them, ((z / T) - max) - log
-// sum, each step rounded to fp32. Equal ones take the mean of the two sides. 117 us for 2044 x 32768 fp32 (105% of the copy
-// rate), 75 us for 508 x 151936 bf16 (94%).
+// The gradient from the row's statistics, elementwise. 117 us for 2044 x 32768 fp32 (105% of the copy rate), 70 us for 508 x
+// 151936 bf16 (101%).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, int64_t ldq, const T* target, int64_t ldp,
-                                                              int64_t rows, int V, float kl, float temp,
+                                                              int64_t rows, int V, float kl, float inv_t,
                                                               const AcceptRow* stats, const float* g_alpha,
                                                               const float* g_kl, T* out, int64_t out_ld) {
   constexpr int N = Vec<T>::N;
@@ -1303,33 +1309,24 @@ __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, in
   load_unit(s, target + row * ldp, xp);
   const AcceptRow st = stats[row];
   const bool nothing = st.fq == 0.f;
-  const float ga = g_alpha[row] / temp, gk = g_kl[row] / temp;
-  const float under = st.fq * (ga * (1.f - st.a) + gk), over = st.fq * (gk - ga * st.a), even = 0.5f * (under + over);
-  const Two k2 = two(kl), bq = two(-st.bq), bp = two(-st.bp), kp = two(-gk * st.fp);
-  const auto unit = [&](auto cold) {
-    store_unit<kPairVec>(s, out + row * out_ld, [&](int i) {
-      float q[N], p[N];
-      Vec<T>::unpack(xq[i], q);
-      Vec<T>::unpack(xp[i], p);
+  const float ga = g_alpha[row] * inv_t, gk = g_kl[row] * inv_t;
+  const Two jump = two(st.fq * ga), rest = two(st.fq * (gk - ga * st.a)), kp = two(-gk * st.fp);
+  const Two k2 = two(kl), bq = two(-st.bq), bp = two(-st.bp);
+  store_unit<kPairVec>(s, out + row * out_ld, [&](int i) {
+    float q[N], p[N];
+    Vec<T>::unpack(xq[i], q);
+    Vec<T>::unpack(xp[i], p);
 #pragma unroll
-      for (int k = 0; k < N; k += 2) {
-        float side[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float zq = cold ? __fdiv_rn(q[k + j], temp) : q[k + j], zp = cold ? __fdiv_rn(p[k + j], temp) : p[k + j];
-          const float lq = __fsub_rn(__fsub_rn(zq, st.mq), st.lq), lp = __fsub_rn(__fsub_rn(zp, st.mp), st.lp);
-          side[j] = lq < lp ? under : lq == lp ? even : over;
-        }
-        const Two eq = fma2(two(q[k], q[k + 1]), k2, bq), ep = fma2(two(p[k], p[k + 1]), k2, bp);
-        const float2 g = halves(fma2(ex2_two(eq), two(side[0], side[1]), mul2(kp, ex2_two(ep))));
-        q[k] = nothing ? 0.f : g.x;
-        q[k + 1] = nothing ? 0.f : g.y;
-      }
-      return Vec<T>::pack(q);
-    });
-  };
-  if (temp == 1.f) unit(std::false_type());
-  else unit(std::true_type());
+    for (int k = 0; k < N; k += 2) {
+      const Two zq = two(q[k], q[k + 1]), zp = two(p[k], p[k + 1]);
+      const float2 h = share2(zq, zp, st.steep, st.middle);
+      const float2 g = halves(fma2(ex2_two(fma2(zq, k2, bq)), fma2(two(h.x, h.y), jump, rest),
+                                   mul2(kp, ex2_two(fma2(zp, k2, bp)))));
+      q[k] = nothing ? 0.f : g.x;
+      q[k + 1] = nothing ? 0.f : g.y;
+    }
+    return Vec<T>::pack(q);
+  });
 }
 
 // ------------------------------------------------------------------------------------------- draft verification
@@ -1826,7 +1823,7 @@ cudaError_t accept_kl(Type type, Logits draft, Logits target, int64_t rows, int 
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     return launch(accept_kernel<T>, s, stream, static_cast<const T*>(draft.p), draft.ld, static_cast<const T*>(target.p),
-                  target.ld, V, p.keep, (float)(kLog2ed / temp), temp, alpha, kl, reinterpret_cast<AcceptRow*>(stats));
+                  target.ld, V, p.keep, (float)(kLog2ed / temp), alpha, kl, reinterpret_cast<AcceptRow*>(stats));
   });
 }
 cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, int V, float temp, const float* stats,
@@ -1837,7 +1834,7 @@ cudaError_t accept_kl_bwd(Type type, Logits draft, Logits target, int64_t rows, 
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     return launch(accept_bwd_kernel<T>, s, stream, static_cast<const T*>(draft.p), draft.ld,
-                  static_cast<const T*>(target.p), target.ld, rows, V, (float)(kLog2ed / temp), temp,
+                  static_cast<const T*>(target.p), target.ld, rows, V, (float)(kLog2ed / temp), 1.f / temp,
                   reinterpret_cast<const AcceptRow*>(stats), g_alpha, g_kl, static_cast<T*>(out), out_ld);
   });
 }

@@ -12,7 +12,7 @@ enum Type { F32 = 0, F16 = 1, BF16 = 2 };
 constexpr int kMaxK = 128;       // teacher tokens per row, drafts per sequence
 constexpr int kMaxV = 1 << 20;
 constexpr int kKdStats = 4;      // floats of per-row state between kd_topk and kd_topk_bwd
-constexpr int kAcceptStats = 9;  // floats of per-row state between accept_kl and accept_kl_bwd
+constexpr int kAcceptStats = 7;  // floats of per-row state between accept_kl and accept_kl_bwd
 
 struct Logits {
   const void* p;

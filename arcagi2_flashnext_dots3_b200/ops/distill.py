@@ -170,8 +170,10 @@ def _accept_cpu(draft, target, t, g_alpha=None, g_kl=None):
         kl = torch.where(p > 0, p * (lp - lq), 0.0)
         kl = torch.where(torch.isnan(p), p, kl).sum(-1)
         return torch.where(nothing, 0.0, torch.minimum(q, p).sum(-1)), torch.where(nothing, 0.0, kl)
-    h = (lq < lp).float() + 0.5 * (lq == lp).float()
-    d = (g_alpha / t)[:, None] * q * (h - (q * h).sum(-1, keepdim=True)) + (g_kl / t)[:, None] * (q - p)
+    # h - A of a token from the masses of the other sides: a sure token's 1 - A is lost in a difference
+    below, even, above = ((q * on).sum(-1, keepdim=True) for on in (lq < lp, lq == lp, lq > lp))
+    h_a = torch.where(lq < lp, above + 0.5 * even, torch.where(lq == lp, 0.5 * (above - below), -(below + 0.5 * even)))
+    d = (g_alpha / t)[:, None] * q * h_a + (g_kl / t)[:, None] * (q - p)
     return torch.where(nothing[:, None], 0.0, d).to(draft.dtype)
 
 
@@ -192,7 +194,7 @@ def accept_kl(draft: torch.Tensor, target: torch.Tensor, temperature: float = 1.
     """(alpha, kl) fp32 [rows] of draft logits against target logits of the same shape and type: alpha = sum_v
     min(q_v, p_v), the probability that speculative verification accepts a token drawn from q, and kl = KL(p || q),
     with q, p the softmaxes at `temperature`. Differentiable in the draft; the target is taken as given. Where q_v =
-    p_v the gradient of alpha is the mean of its two sides. A row in which either side has no token left gives zeros."""
+    p_v (for the kernels: to within a few fp32 roundings) the gradient of alpha is the mean of its two sides. A row in which either side has no token left gives zeros."""
     if draft.is_cuda:
         return native.C().accept_kl(draft, target, temperature)
     draft = _rows(draft, "draft logits")
