@@ -435,26 +435,6 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
   return __uint_as_float((ord & 0x80000000u) ? (ord ^ 0x80000000u) : ~ord);
 }
 
-// A warp's part of a unit: its threads share their offset, so it is one maximum and one sum. `m`: the thread's largest logit,
-// or kFloor.
-template <typename T, int kVec>
-__device__ __forceinline__ Soft warp_soft(const uint4 (&x)[kVec], float m, float kl) {
-  constexpr int N = Vec<T>::N;
-  const float c = warp_reduce(m, Max()) * kl;
-  const Two k2 = two(kl), c2 = two(-c);
-  Two a = two(0.f), b = two(0.f);
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    float f[N];
-    Vec<T>::unpack(x[i], f);
-#pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      a = add2(a, ex2_two(fma2(two(f[k], f[k + 1]), k2, c2)));
-      b = add2(b, ex2_two(fma2(two(f[k + 2], f[k + 3]), k2, c2)));
-    }
-  }
-  return {c, warp_reduce(sum(add2(a, b)), Add())};
-}
 template <typename T, int kVec>
 __device__ __forceinline__ float unit_max(const uint4 (&x)[kVec]) {
   if constexpr (sizeof(T) == 4) {
@@ -1335,12 +1315,58 @@ __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, in
 // parts, finds the first rejected draft and draws from that position alone: the race costs a hash per token and is run for
 // one row of the k + 1. A draw needs -log(u) / r below the best so far; -log(u) >= 1 - u, which is the hash's integer, so
 // the logarithm and the division are taken for the few tokens that can win.
-// 54 us for 64 sequences of 3 soft drafts x 151936 bf16: 30 us the rows (70% of the copy rate), 24 us the draw, bound by the 48
-// instructions per token, most of them the hash's 64-bit products. 34 us for 32 sequences of up to 7 point-mass drafts x
-// 152064 fp32 (70% of the copy rate over both). One sequence of 3: 10 us, latency.
+// 55.5 us for 64 sequences of 3 soft drafts x 151936 bf16: 31 us the rows (68% of the copy rate), 24 us the draw, bound by the 50
+// instructions per token, most of them the hash's 64-bit products. 34.6 us for 32 sequences of up to 7 point-mass drafts x
+// 152064 fp32 (69% of the copy rate over both). One sequence of 3: 10 us, latency.
 constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr int kDrawVec = 2;          // vectors that a thread requests at once
+
+// Temperatures come with requests, from next to nothing to infinity. kl stays finite; at T = 1e20 all logits weigh the same to fp32,
+// and a masked one still nothing. An offset m kl rounded once would be off by more than 2^127 from a T of some 1e-7 down, so
+// here the largest logit is taken off first and the rest scaled: one more operation per logit (54.0 -> 55.5 us for 64 sequences
+// of 3 soft drafts x 151936 bf16).
+__device__ __forceinline__ float scale_of(float temp) { return fminf(kLog2e / fminf(temp, 1e20f), 3e38f); }
+// sum = sum over elements of 2^((z - m) kl), m the largest z or kFloor
+struct Peak {
+  float m, sum;
+};
+__device__ __forceinline__ Peak join(Peak a, Peak b, float kl) {
+  const float m = fmaxf(a.m, b.m);
+  return {m, a.sum * ex2((a.m - m) * kl) + b.sum * ex2((b.m - m) * kl)};
+}
+__device__ __forceinline__ Peak as_peak(unsigned long long u) {
+  return {__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32))};
+}
+// A warp's part of a unit: its threads share their maximum. `top`: the thread's largest logit.
+template <typename T, int kVec>
+__device__ __forceinline__ Peak warp_peak(const uint4 (&x)[kVec], float top, float kl) {
+  constexpr int N = Vec<T>::N;
+  const float m = warp_reduce(fmaxf(top, kFloor), Max());
+  const Two k2 = two(kl), m2 = two(-m);
+  Two a = two(0.f), b = two(0.f);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    float f[N];
+    Vec<T>::unpack(x[i], f);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      a = add2(a, ex2_two(mul2(add2(two(f[k], f[k + 1]), m2), k2)));
+      b = add2(b, ex2_two(mul2(add2(two(f[k + 2], f[k + 3]), m2), k2)));
+    }
+  }
+  return {m, warp_reduce(sum(add2(a, b)), Add())};
+}
+// Joins a list of parts over a warp, as join_parts does.
+template <typename Load>
+__device__ __forceinline__ Peak join_peaks(int n, float kl, Load load) {
+  Peak t{kFloor, 0.f};
+  for (int i = threadIdx.x & 31; i < n; i += 32) t = join(t, as_peak(load(i)), kl);
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    t = join(t, Peak{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.sum, o)}, kl);
+  return t;
+}
 
 constexpr uint64_t kIndexStep = 0x8CB92BA72F3D8DD7ull;
 // x * c modulo 2^64 in 32-bit halves
@@ -1366,7 +1392,7 @@ __device__ __forceinline__ int drafts_of(const Verify& a, int64_t b) {
 }
 
 // Workspace: best draw and arrivals of each sequence, then parts [batch][2 k + 1 rows: k + 1 of the target, k of the
-// draft][splits], 8 bytes each: Soft, or a rank_key.
+// draft][splits], 8 bytes each: Peak, or a rank_key.
 __device__ __forceinline__ unsigned long long* verify_best(const Verify& a) {
   return static_cast<unsigned long long*>(a.workspace);
 }
@@ -1415,13 +1441,13 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
     __syncthreads();
     for (int w = 0; w < kWarps; ++w) res = min(res, warp_part[w]);
   } else {
-    const float kl = kLog2e / temp;
-    const Soft soft = warp_soft<T>(x, fmaxf(top, kFloor), kl);
-    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = as_u64(soft.c, soft.sum);
+    const float kl = scale_of(temp);
+    const Peak part = warp_peak<T>(x, top, kl);
+    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = as_u64(part.m, part.sum);
     __syncthreads();
     if (threadIdx.x >= 32) return;
-    const Soft t = join_parts(kWarps, kl, [&](int i) { return warp_part[i]; });
-    res = as_u64(t.c, t.sum);
+    const Peak t = join_peaks(kWarps, kl, [&](int i) { return warp_part[i]; });
+    res = as_u64(t.m, t.sum);
   }
   if (threadIdx.x == 0) verify_parts(a)[blockIdx.x] = res;
 }
@@ -1429,7 +1455,7 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
 template <typename T>
 __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, int splits, int blocks, int per) {
   constexpr int N = Vec<T>::N;
-  __shared__ Soft s_p[kMaxK + 1], s_q[kMaxK];
+  __shared__ Peak s_p[kMaxK + 1], s_q[kMaxK];
   __shared__ unsigned long long s_best[kMaxK + 1];
   __shared__ int s_ok[kMaxK + 1];
   __shared__ unsigned long long warp_best[kDrawWarps];
@@ -1442,7 +1468,7 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
   const int n = drafts_of(a, b);
   const float temp = a.temps[b];
   const bool greedy = !(temp > 0.f);
-  const float kl = greedy ? 1.f : kLog2e / temp;
+  const float kl = greedy ? 1.f : scale_of(temp);
   const uint64_t seed = (uint64_t)a.seeds[b] * 0x9E3779B97F4A7C15ull + 1ull, step = (uint64_t)a.steps[b];
   const unsigned long long* parts = verify_parts(a) + b * rows * splits;
   for (int j = tid >> 5; j <= n; j += kDrawWarps) {     // one warp per position
@@ -1460,19 +1486,19 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
       }
       continue;
     }
-    const auto whole = [&](int r) { return join_parts(splits, kl, [&](int i) { return parts[r * splits + i]; }); };
-    const Soft p = whole(j), q = a.draft_logits && j < n ? whole(a.k + 1 + j) : Soft{0.f, 1.f};
+    const auto whole = [&](int r) { return join_peaks(splits, kl, [&](int i) { return parts[r * splits + i]; }); };
+    const Peak p = whole(j), q = a.draft_logits && j < n ? whole(a.k + 1 + j) : Peak{0.f, 1.f};
     if (lane == 0) {
       s_p[j] = p;
       if (j < n) s_q[j] = q;
       bool ok = false;
       if (known) {
         const float zp = Vec<T>::one(static_cast<const T*>(a.logits)[b * a.logits_b + j * a.logits_j + id]);
-        const float pd = p.sum > 0.f ? ex2(fmaf(zp, kl, -p.c)) / p.sum : 0.f;
+        const float pd = p.sum > 0.f ? ex2((zp - p.m) * kl) / p.sum : 0.f;
         float qd = 1.f;
         if (a.draft_logits) {
           const float zq = Vec<T>::one(static_cast<const T*>(a.draft_logits)[b * a.draft_b + j * a.draft_j + id]);
-          qd = q.sum > 0.f ? ex2(fmaf(zq, kl, -q.c)) / q.sum : 0.f;
+          qd = q.sum > 0.f ? ex2((zq - q.m) * kl) / q.sum : 0.f;
         }
         ok = unit(random23(seed + (step + j) * 0xD1B54A32D192ED03ull - kIndexStep)) * qd < pd;   // index -1
       }
@@ -1493,8 +1519,8 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
   const T* qrow = a.draft_logits && acc < n ? static_cast<const T*>(a.draft_logits) + b * a.draft_b + acc * a.draft_j : nullptr;
   const int64_t id = acc >= n ? -1 : a.wide ? static_cast<const int64_t*>(a.drafts)[b * a.k + acc]
                                             : (int64_t) static_cast<const int32_t*>(a.drafts)[b * a.k + acc];
-  const Soft p = s_p[acc];
-  const float ip = 1.f / p.sum, cq = qrow ? s_q[acc].c : 0.f, iq = qrow && s_q[acc].sum > 0.f ? 1.f / s_q[acc].sum : 0.f;
+  const Peak p = s_p[acc];
+  const float ip = 1.f / p.sum, mq = qrow ? s_q[acc].m : 0.f, iq = qrow && s_q[acc].sum > 0.f ? 1.f / s_q[acc].sum : 0.f;
   const bool same = ((reinterpret_cast<uintptr_t>(qrow) ^ reinterpret_cast<uintptr_t>(row)) & 15) == 0;
   const uint64_t base = seed + (step + acc) * 0xD1B54A32D192ED03ull;
   // The earliest of all times is exponential with the rate sum r: 1 for p, 1 - p(d) beside a point mass. A draw that only
@@ -1504,7 +1530,7 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
   // limit, and, if the residual is empty, over p itself.
   float limit = 24.f;
   if (qrow) limit = 1024.f;
-  else if (id >= 0 && id < a.V) limit = 24.f / fmaxf(1.f - ex2(fmaf(Vec<T>::one(row[id]), kl, -p.c)) * ip, 1e-6f);
+  else if (id >= 0 && id < a.V) limit = 24.f / fmaxf(1.f - ex2((Vec<T>::one(row[id]) - p.m) * kl) * ip, 1e-6f);
   for (int stage = 0;; ++stage) {
     const bool whole = acc == n || stage == 2;
     const Slice<T> s(row, a.V, stage ? a.V : per, stage ? 0 : rank);
@@ -1537,9 +1563,9 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
             uint32_t h[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k, counter += kIndexStep) {
-              r[k] = ex2(fmaf(f[k0 + k], kl, -p.c)) * ip;
+              r[k] = ex2((f[k0 + k] - p.m) * kl) * ip;
               if (residual == 1 && i0 + k0 + k == id) r[k] = 0.f;
-              if (residual == 2) r[k] = fmaf(ex2(fmaf(g[k0 + k], kl, -cq)), -iq, r[k]);
+              if (residual == 2) r[k] = fmaf(ex2((g[k0 + k] - mq) * kl), -iq, r[k]);
               // u = (h + 1/2) 2^-23; -log(u) > 1 - u > 1 - (h + 1) 2^-23, exact from 1 + h 2^-23
               h[k] = random23(counter);
               const float miss = (2.f - 0x1p-23f) - __uint_as_float(0x3F800000u | h[k]);

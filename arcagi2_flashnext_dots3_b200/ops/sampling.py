@@ -224,7 +224,8 @@ def speculative_verify(logits: torch.Tensor, drafts: torch.Tensor, temps: torch.
     noise of (seed, step + j, token) they would otherwise share. ``n_draft`` int32 [B]: drafts of each sequence, 0 to
     k; later positions are not read.
 
-    T <= 0 is greedy: accepted while the draft is the argmax (lowest id on ties), which is also the next token. A draft
+    Any temperature goes: the largest logit is taken off before the division, so a T next to 0 keeps the largest logits alone,
+    and beyond 1e20 all unmasked tokens weigh the same. T <= 0 is greedy: accepted while the draft is the argmax (lowest id on ties), which is also the next token. A draft
     outside the vocabulary is rejected. Masked logits (at or below -1e30) are never drawn; a residual that is empty in
     fp32 draws from p; a position with no token left gives -1."""
     if logits.is_cuda:
@@ -251,9 +252,9 @@ def speculative_verify(logits: torch.Tensor, drafts: torch.Tensor, temps: torch.
 
 def _probabilities(row: torch.Tensor, T: float) -> torch.Tensor:
     z = row.float()
-    z = z.masked_fill(z <= -1e30, float("-inf")) / T
+    z = z.masked_fill(z <= -1e30, float("-inf"))
     m = z.max()
-    return torch.zeros_like(z) if m == float("-inf") else torch.softmax(z, -1)
+    return torch.zeros_like(z) if m == float("-inf") else torch.softmax((z - m) / min(T, 1e20), -1)
 
 
 def _verify_one(lg: torch.Tensor, drafts: list, T: float, seed: int, step: int, draft_lg=None):
