@@ -423,9 +423,12 @@ struct MinKey {
   }
 };
 
-// (value, index) ordered by value descending, then index ascending, as an increasing 64-bit key; ~0 is no entry.
+// (value, index) ordered by value descending, then index ascending, as an increasing 64-bit key above 0; any NaN ranks above all
+// numbers. ~0 is no entry, and key_value of it is a NaN.
 constexpr unsigned long long kNone = ~0ull;
+constexpr unsigned long long kNanKey = 1ull << 32;
 __device__ __forceinline__ unsigned long long rank_key(float v, uint32_t i) {
+  if (isnan(v)) return kNanKey | i;
   const uint32_t u = __float_as_uint(v + 0.f);   // -0 ranks with +0
   const uint32_t ord = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return ((unsigned long long)~ord << 32) | i;
@@ -523,7 +526,8 @@ __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, i
   Soft soft{kFloor * kl, 0.f};
   uint4 x[kUnit];
   load_unit(s, x);
-  tops[unit_index() * kThreads + tid] = add_soft<T>(x, kl, m, soft);
+  const float top = add_soft<T>(x, kl, m, soft);
+  tops[unit_index() * kThreads + tid] = isnan(soft.sum) ? INFINITY : top;     // a NaN (or +inf) among them: to be looked at
 #pragma unroll
   for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
   if ((tid & 31) == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
@@ -590,13 +594,11 @@ __global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, 
   const auto look = [&](int from, int i, auto visit) {
     const int at = s.start(((from >> 8) * kUnit + i) * kThreads + (from & 255));
     const uint4 x = s.full(at) ? __ldcg(reinterpret_cast<const uint4*>(s.row + at)) : ragged_vec(s, s.row, at);
-    if (packed_max<T>(x) >= bound) {
-      float f[N];
-      Vec<T>::unpack(x, f);
+    float f[N];
+    Vec<T>::unpack(x, f);
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (f[j] >= bound) visit(rank_key(f[j], at + j));
-    }
+    for (int j = 0; j < N; ++j)
+      if (!(f[j] < bound)) visit(rank_key(f[j], at + j));          // a NaN too
   };
   const int listed = s_listed;
   if (listed <= kCand)

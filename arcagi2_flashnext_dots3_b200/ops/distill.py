@@ -66,7 +66,8 @@ def _log_softmax(x: torch.Tensor, t: float) -> torch.Tensor:
 def teacher_topk(logits: torch.Tensor, k: int, temperature: float = 1.0):
     """(ids int32 [rows, k], log-probabilities fp32 [rows, k]) of the k largest logits of each row, best first (ties:
     lowest id), under softmax(logits / temperature). Rows with fewer than k unmasked tokens are padded with id -1 and
-    log-probability -inf, the padding of the distillation records. k <= 128."""
+    log-probability -inf, the padding of the distillation records. A NaN ranks above every number and makes the row's
+    log-probabilities NaN. k <= 128."""
     if logits.is_cuda:
         return native.C().teacher_topk(logits, k, temperature)
     logits = _rows(logits.detach(), "logits")
@@ -76,9 +77,10 @@ def teacher_topk(logits: torch.Tensor, k: int, temperature: float = 1.0):
     n, V = logits.shape
     ls = _log_softmax(logits, t)
     z = logits.float()
-    order = torch.sort(z.masked_fill(z <= MASKED, float("-inf")), dim=-1, descending=True, stable=True).indices[:, :k]
-    lp = ls.gather(1, order)
-    ids = order.to(torch.int32).masked_fill(lp == float("-inf"), -1)
+    z, order = torch.sort(z.masked_fill(z <= MASKED, float("-inf")), dim=-1, descending=True, stable=True)
+    z, order = z[:, :k], order[:, :k]
+    lp = ls.gather(1, order).masked_fill(z == float("-inf"), float("-inf"))
+    ids = order.to(torch.int32).masked_fill(z == float("-inf"), -1)
     if k > V:
         ids = torch.cat([ids, ids.new_full((n, k - V), -1)], 1)
         lp = torch.cat([lp, lp.new_full((n, k - V), float("-inf"))], 1)
