@@ -456,6 +456,29 @@ __device__ __forceinline__ float unit_max(const uint4 (&x)[kVec]) {
     return fmaxf(Vec<T>::one(m.x), Vec<T>::one(m.y));
   }
 }
+// Whether the vectors hold a NaN, which the maxima above drop.
+template <typename T, int kVec>
+__device__ __forceinline__ bool unit_nan(const uint4 (&x)[kVec]) {
+  if constexpr (sizeof(T) == 4) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      float f[4];
+      Vec<T>::unpack(x[i], f);
+      nan |= isnan(f[0]) | isnan(f[1]) | isnan(f[2]) | isnan(f[3]);
+    }
+    return nan;
+  } else {
+    using T2 = typename Vec<T>::Pair;
+    T2 m = *reinterpret_cast<const T2*>(&x[0]);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const T2* p = reinterpret_cast<const T2*>(&x[i]);
+      m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3])));
+    }
+    return isnan(Vec<T>::one(m.x)) || isnan(Vec<T>::one(m.y));
+  }
+}
 // Adds vectors to a thread's running softmax with maximum m; returns their largest logit.
 template <typename T, int kVec>
 __device__ __forceinline__ float add_soft(const uint4 (&x)[kVec], float kl, float& m, Soft& s) {
@@ -1318,8 +1341,8 @@ __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, in
 // one row of the k + 1. A draw needs -log(u) / r below the best so far; -log(u) >= 1 - u, which is the hash's integer, so
 // the logarithm and the division are taken for the few tokens that can win.
 // 55.5 us for 64 sequences of 3 soft drafts x 151936 bf16: 31 us the rows (68% of the copy rate), 24 us the draw, bound by the 50
-// instructions per token, most of them the hash's 64-bit products. 34.6 us for 32 sequences of up to 7 point-mass drafts x
-// 152064 fp32 (69% of the copy rate over both). One sequence of 3: 10 us, latency.
+// instructions per token, most of them the hash's 64-bit products. 34.9 us for 32 sequences of up to 7 point-mass drafts x
+// 152064 fp32 (68% of the copy rate over both). One sequence of 3: 10 us, latency.
 constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr int kDrawVec = 2;          // vectors that a thread requests at once
@@ -1402,7 +1425,7 @@ __device__ __forceinline__ unsigned long long* verify_count(const Verify& a) { r
 __device__ __forceinline__ unsigned long long* verify_parts(const Verify& a) { return verify_best(a) + 2 * a.batch; }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int splits) {
+__global__ void __launch_bounds__(kThreads, 5) verify_parts_kernel(Verify a, int splits) {
   constexpr int N = Vec<T>::N;
   __shared__ unsigned long long warp_part[kWarps];
   const int rows = a.draft_logits ? 2 * a.k + 1 : a.k + 1;
@@ -1438,6 +1461,7 @@ __global__ void __launch_bounds__(kThreads) verify_parts_kernel(Verify a, int sp
           if (f[k] == best) res = rank_key(best, s.start(threadIdx.x + i * kThreads) + k);
       }
     }
+    if (unit_nan<T>(x)) res = kNanKey;
     res = warp_reduce(res, MinKey());
     if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = res;
     __syncthreads();
@@ -1482,6 +1506,7 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
       unsigned long long best = kNone;
       for (int i = lane; i < splits; i += 32) best = min(best, parts[j * splits + i]);
       best = warp_reduce(best, MinKey());
+      if (isnan(key_value(best))) best = kNone;
       if (lane == 0) {
         s_best[j] = best;
         s_ok[j] = known && best != kNone && (uint32_t)best == (uint32_t)id;
@@ -1500,7 +1525,7 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
         float qd = 1.f;
         if (a.draft_logits) {
           const float zq = Vec<T>::one(static_cast<const T*>(a.draft_logits)[b * a.draft_b + j * a.draft_j + id]);
-          qd = q.sum > 0.f ? ex2((zq - q.m) * kl) / q.sum : 0.f;
+          qd = q.sum == 0.f ? 0.f : ex2((zq - q.m) * kl) / q.sum;        // NaN in the row: NaN, and the draft is rejected
         }
         ok = unit(random23(seed + (step + j) * 0xD1B54A32D192ED03ull - kIndexStep)) * qd < pd;   // index -1
       }
@@ -1534,7 +1559,7 @@ __global__ void __launch_bounds__(kDrawThreads, 5) verify_draw_kernel(Verify a, 
   if (qrow) limit = 1024.f;
   else if (id >= 0 && id < a.V) limit = 24.f / fmaxf(1.f - ex2((Vec<T>::one(row[id]) - p.m) * kl) * ip, 1e-6f);
   for (int stage = 0;; ++stage) {
-    const bool whole = acc == n || stage == 2;
+    const bool whole = acc == n || stage == 2 || (qrow && isnan(s_q[acc].sum));
     const Slice<T> s(row, a.V, stage ? a.V : per, stage ? 0 : rank);
     unsigned long long best = kNone;
     float bound = stage ? INFINITY : limit;                           // of this warp: the limit, then its best time

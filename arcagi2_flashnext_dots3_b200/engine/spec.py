@@ -152,9 +152,9 @@ class SpecGraph:
             drafts = self.ids[:, 1:].contiguous()
             acc, nxt = sampling.speculative_verify(m.logits(x).view(B, k1, -1), drafts, self.temps, self.seeds, self.steps)
             at = torch.arange(k1, device=x.device)[None]
-            # y[j] is draft j while it was accepted, then the drawn token (0 where nothing could be drawn: no logit left)
+            # y[j] is draft j while it was accepted, then the drawn token; the host looks for -1, the head takes 0 for it
             y = torch.where(at < acc[:, None], torch.cat([drafts, nxt[:, None]], 1),
-                            torch.where(at == acc[:, None], nxt[:, None], 0)).clamp_min(0)
+                            torch.where(at == acc[:, None], nxt[:, None], 0))
         else:
             y = greedy_ids(m, x).view(B, k1)
             match = (self.ids[:, 1:] == y[:, :k]).to(torch.int32)
@@ -162,6 +162,7 @@ class SpecGraph:
         m.commit(acc + 1)
         self.y.copy_(y)
         self.acc.copy_(acc)
+        y = y.clamp_min(0)
         if self.head is not None:
             h = self.head
             xm = h.step(x, y.reshape(-1), self.slots, self.pos, k1)
@@ -193,6 +194,12 @@ class SpecGraph:
 
     def run(self):
         self.graph.replay()
+
+
+def _check_drawn(tokens):
+    """speculative_verify gives -1 where it has no token to give: logits that are NaN, or all masked."""
+    if min(tokens) < 0:
+        raise RuntimeError("no token could be drawn from the model's logits (NaN, or nothing unmasked)")
 
 
 class SpecDecoder:
@@ -246,6 +253,7 @@ class SpecDecoder:
         out = torch.cat([g.y, g.acc[:, None], g.nd], 1).cpu()
         y = out[:n, :k1].tolist()
         accepted = out[:n, k1].tolist()
+        _check_drawn([row[a] for row, a in zip(y, accepted)])
         if head is not None:
             for s, row in zip(seqs, out[:n, k1 + 1:].tolist()):
                 self.drafter.next[s.slot] = row
@@ -305,7 +313,9 @@ class SpecDecoder:
             t = [torch.tensor(v, dtype=ty).to(lg.device) for v, ty in
                  ((temps, torch.float32), (seeds, torch.int64), (steps, torch.int64))]
             acc, nxt = sampling.speculative_verify(lg, dr.to(lg.device), *t)
-            return acc.tolist(), nxt.clamp_min(0).tolist()         # -1: no logit left to draw
+            nxt = nxt.tolist()
+            _check_drawn(nxt)
+            return acc.tolist(), nxt
         return sampling.speculative_accept(lg.float(), dr, temps, seeds, steps)
 
     def _advance(self, seqs, drafts, y, accepted) -> dict:
