@@ -670,7 +670,10 @@ __global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, 
 struct KdRow {
   float c, inv_s, ratio, csum;   // softmax offset and 1 / sum (0: nothing in the row), tt / ts (0 at the floor), sum c
 };
-static_assert(sizeof(KdRow) == kKdStats * 4, "KdRow is what callers allocate");
+struct KdSaved {
+  float c, inv_s, pull, csum;    // of a KdRow, and pull_of
+};
+static_assert(sizeof(KdSaved) == kKdStats * 4, "KdSaved is what callers allocate");
 
 // Whether entry i of the row's teacher ids repeats an earlier one.
 __device__ __forceinline__ bool repeats(const int* ids, int i) {
@@ -794,10 +797,15 @@ __device__ __forceinline__ float kd_loss(const TeacherSums& e, const Soft& tail)
   if (e.mass != 0.0) l += e.mass * kLn2d * ((double)c - e.c + log2(total));
   return (float)l;
 }
-// w d loss / d z at a teacher's token
-__device__ __forceinline__ float kd_pull(const KdRow& r, float w, float z, float pt, float kl) {
-  const float ps = ex2(fmaf(z, kl, -r.c)) * r.inv_s;
-  return r.inv_s == 0.f ? 0.f : w * fmaf(r.ratio - r.csum, ps, -pt);
+// The gradient at a teacher's token is w (c_k - ps sum c) = w (pull ps - pt) with pull = tt / ts - sum c = tt / ts (1 - sum ps) + sum
+// pt, that is tt + sum pt, without tt at the floor. Formed as the difference it loses the tail of a sure student (ts = 1e-6: 0.06
+// of a gradient of 0.3).
+__device__ __forceinline__ float pull_of(const TeacherSums& e, float ratio) {
+  return (float)e.mass + (ratio > 0.f ? e.tt : 0.f);
+}
+__device__ __forceinline__ float kd_pull(float c, float inv_s, float pull, float w, float z, float pt, float kl) {
+  const float ps = ex2(fmaf(z, kl, -c)) * inv_s;
+  return inv_s == 0.f ? 0.f : w * fmaf(pull, ps, -pt);
 }
 
 // A vector with -inf in element j.
@@ -871,7 +879,7 @@ __global__ void __launch_bounds__(kThreads) kd_parts_kernel(const T* logits, int
 
 template <typename T>
 __global__ void __launch_bounds__(32) kd_loss_kernel(const T* logits, int64_t ld, int splits, int V, Teacher t, float kl,
-                                                     const unsigned long long* parts, float* loss, KdRow* stats) {
+                                                     const unsigned long long* parts, float* loss, KdSaved* stats) {
   __shared__ int s_id[kMaxK];
   const int64_t row = blockIdx.x;
   pdl_launch_dependents();
@@ -884,7 +892,10 @@ __global__ void __launch_bounds__(32) kd_loss_kernel(const T* logits, int64_t ld
   const Soft tail = join_parts(splits, kl, [&](int i) { return parts[row * splits + i]; });
   if (threadIdx.x == 0) {
     loss[row] = kd_loss(sums, tail);
-    if (stats) stats[row] = kd_finish(sums, tail);
+    if (stats) {
+      const KdRow f = kd_finish(sums, tail);
+      stats[row] = KdSaved{f.c, f.inv_s, pull_of(sums, f.ratio), f.csum};
+    }
   }
 }
 
@@ -1050,7 +1061,8 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) kd_grad_kernel(const 
     o[single] = *reinterpret_cast<const T*>(&x);
   }
   for (int j = 0; j < listed; ++j)
-    if (s.owns(list.id[j]) || list.id[j] == single) o[list.id[j]] = Vec<T>::back(kd_pull(f, w, list.z[j], list.pt[j], kl));
+    if (s.owns(list.id[j]) || list.id[j] == single)
+      o[list.id[j]] = Vec<T>::back(kd_pull(f.c, f.inv_s, pull_of(e, f.ratio), w, list.z[j], list.pt[j], kl));
 }
 
 // The gradient from statistics, elementwise; `out` may be the logits. 189 us for 1024 x 151936 fp32, 376 us for 4096 x 152064
@@ -1058,7 +1070,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) kd_grad_kernel(const 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64_t ld, int64_t rows, int V, Teacher t,
                                                           float kl, float inv_t, const float* weight,
-                                                          const KdRow* stats, T* out, int64_t out_ld) {
+                                                          const KdSaved* stats, T* out, int64_t out_ld) {
   const int64_t row = unit_row();
   if (row >= rows) return;
   const Slice<T> s(logits + row * ld, V, kUnit * kThreads, blockIdx.x);
@@ -1070,7 +1082,7 @@ __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64
   if (id >= 0 && s.place(id) < 0) id = -1;
   const float z = id >= 0 ? masked(Vec<T>::one(s.row[id])) : 0.f;
   pdl_wait();
-  const KdRow st = stats[row];
+  const KdSaved st = stats[row];
   const float w = st.inv_s == 0.f ? 0.f : weight[row] * inv_t;
   const Two scale = two(st.inv_s == 0.f ? 0.f : -st.csum * st.inv_s * w), c2 = two(-st.c), k2 = two(kl);
   __syncthreads();                                     // every z is read
@@ -1079,7 +1091,7 @@ __global__ void __launch_bounds__(kThreads) kd_bwd_kernel(const T* logits, int64
   if (id >= 0) {
     bool repeated = false;
     for (int j = 0; j < tid; ++j) repeated |= load_id(t, row * t.k + j, V) == id;
-    if (!repeated) o[id] = Vec<T>::back(kd_pull(st, w, z, expf(t.lp[row * t.k + tid]), kl));
+    if (!repeated) o[id] = Vec<T>::back(kd_pull(st.c, st.inv_s, st.pull, w, z, expf(t.lp[row * t.k + tid]), kl));
   }
 }
 
@@ -1802,7 +1814,7 @@ cudaError_t kd_topk_loss(Type type, Logits z, int64_t rows, int V, Teacher t, fl
     const cudaError_t e = launch(kd_parts_kernel<T>, parts, stream, p, z.ld, rows, V, t, (float)(kLog2ed / temp), words);
     if (e != cudaSuccess) return e;
     return launch(kd_loss_kernel<T>, last, stream, p, z.ld, splits, V, t, (float)(kLog2ed / temp), words, loss,
-                  reinterpret_cast<KdRow*>(stats));
+                  reinterpret_cast<KdSaved*>(stats));
   });
 }
 
@@ -1815,7 +1827,7 @@ static cudaError_t kd_from_stats(Type type, Logits z, int64_t rows, int V, Teach
   return by_type(type, [&](auto x) {
     using T = decltype(x);
     return launch(kd_bwd_kernel<T>, s, stream, static_cast<const T*>(z.p), z.ld, rows, V, t, (float)(kLog2ed / temp),
-                  1.f / temp, weight, reinterpret_cast<const KdRow*>(stats), static_cast<T*>(out), out_ld);
+                  1.f / temp, weight, reinterpret_cast<const KdSaved*>(stats), static_cast<T*>(out), out_ld);
   });
 }
 
@@ -1828,7 +1840,7 @@ static bool kd_in_l2(Type type, int64_t rows, int V) {
   return rows * V * (type == F32 ? 4 : 2) <= l2;
 }
 size_t kd_topk_grad_workspace(Type type, Logits z, int64_t rows, int V, int k) {
-  if (kd_in_l2(type, rows, V)) return rows * sizeof(KdRow) + kd_topk_loss_workspace(type, z, rows, V);
+  if (kd_in_l2(type, rows, V)) return rows * sizeof(KdSaved) + kd_topk_loss_workspace(type, z, rows, V);
   size_t bytes;
   carve_kd(rows, k, nullptr, bytes);
   return bytes;

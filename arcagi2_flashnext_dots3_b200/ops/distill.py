@@ -107,9 +107,10 @@ def _kd_cpu(logits, t_ids, t_lp, t, weight=None):
     loss = torch.where(nothing, 0.0, loss)
     if weight is None:
         return loss
-    ratio = torch.where(tail >= TAIL_FLOOR, tt / ts, 0.0)
-    c = torch.where(valid, -pt + ratio[:, None] * s.exp(), 0.0)
-    d = (-c.sum(-1, keepdim=True) * p).scatter_add(1, at, c)[:, :V] * (weight / t)[:, None]
+    on, mass, ps = tail >= TAIL_FLOOR, pt.sum(-1), torch.where(valid, s.exp(), 0.0)
+    csum = torch.where(on, tt / ts, 0.0) * ps.sum(-1) - mass
+    pull = torch.where(on, tt, 0.0) + mass            # tt / ts - csum, which would lose a sure student's tail as a difference
+    d = (-csum[:, None] * p).scatter(1, at, pull[:, None] * ps - pt)[:, :V] * (weight / t)[:, None]
     return loss, torch.where(nothing[:, None], 0.0, d).to(logits.dtype)
 
 
