@@ -17,12 +17,14 @@ here reads from the host, so every call can be captured in a CUDA graph.
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad
 
 from . import native
 
 MASKED = -1e30       # csrc/k_vocab.cu kFloor is the float above it
 TAIL_FLOOR = 1e-8    # csrc/k_vocab.cu kTailFloor
 MAX_K = 128          # csrc/vocab.h kMaxK
+MAX_V = 1 << 20      # csrc/vocab.h kMaxV
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -60,6 +62,44 @@ def _log_softmax(x: torch.Tensor, t: float) -> torch.Tensor:
     z = z.masked_fill(z <= MASKED, float("-inf")) / t
     nothing = (z == float("-inf")).all(-1, keepdim=True)
     return torch.log_softmax(z.masked_fill(nothing, 0.0), -1).masked_fill(nothing, float("-inf"))
+
+
+def transformed() -> bool:
+    """Whether the caller runs under forward-mode differentiation or a torch.func transform, which the operators here do
+    not take part in."""
+    return torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
+
+
+class _Twice(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, fast, plain):
+        ctx.fast, ctx.plain = fast, plain
+        ctx.save_for_backward(x)
+        ctx.inner = _Twice.run(fast, x)
+        return tuple(o.detach() for o in ctx.inner[1])
+
+    @staticmethod
+    def run(f, x):
+        with torch.enable_grad():
+            z = x.detach().requires_grad_()
+            return z, f(z)
+
+    @staticmethod
+    def backward(ctx, *g):
+        x, = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            return torch.autograd.grad(ctx.plain(x), x, g, create_graph=True)[0], None, None
+        z, out = ctx.inner or _Twice.run(ctx.fast, x)       # the graph that forward left is walked once
+        ctx.inner = None
+        return torch.autograd.grad(out, z, g)[0], None, None
+
+
+def twice(x: torch.Tensor, fast, plain) -> tuple:
+    """fast(x), a tuple of tensors, for callers that may differentiate its gradient again: a backward pass that is itself recorded
+    goes through plain(x), the same in torch operations."""
+    if not (x.requires_grad and torch.is_grad_enabled()):
+        return fast(x)
+    return _Twice.apply(x, fast, plain)
 
 
 # ------------------------------------------------------------------------------------------------ teacher top-k

@@ -162,13 +162,17 @@ def sft_loss(model, ids: torch.Tensor, resp_start: int, chunk: int = 1024) -> to
 def kd_topk_loss(student_logits: torch.Tensor, t_ids: torch.Tensor, t_logprobs: torch.Tensor) -> torch.Tensor:
     """KL(teacher || student) over the teacher's top-k tokens plus one tail bin (the reference's 21-bin top-20
     KL, flashnext/training/kd/train_kd.py). student_logits [n, V]; t_ids, t_logprobs [n, k]."""
-    if student_logits.dim() == 2 and student_logits.dtype in distill.DTYPES and t_ids.shape[-1] <= distill.MAX_K and \
-            not t_logprobs.requires_grad:
-        return distill.kd_topk(student_logits, t_ids.long(), t_logprobs).mean()
-    ls = torch.log_softmax(student_logits.float(), -1)
-    ps_top = ls.gather(-1, t_ids.long())
-    pt_top = t_logprobs.float().exp()
-    tail_t = (1 - pt_top.sum(-1)).clamp_min(1e-8)
-    tail_s = (1 - ps_top.exp().sum(-1)).clamp_min(1e-8)
-    kl = (pt_top * (t_logprobs.float() - ps_top)).sum(-1) + tail_t * (tail_t.log() - tail_s.log())
-    return kl.mean()
+    def plain(logits):
+        ls = torch.log_softmax(logits.float(), -1)
+        ps_top = ls.gather(-1, t_ids.long())
+        pt_top = t_logprobs.float().exp()
+        tail_t = (1 - pt_top.sum(-1)).clamp_min(1e-8)
+        tail_s = (1 - ps_top.exp().sum(-1)).clamp_min(1e-8)
+        return (pt_top * (t_logprobs.float() - ps_top)).sum(-1) + tail_t * (tail_t.log() - tail_s.log()),
+
+    if student_logits.dim() != 2 or student_logits.dtype not in distill.DTYPES or \
+            not 1 <= student_logits.shape[-1] <= distill.MAX_V or not 1 <= t_ids.shape[-1] <= distill.MAX_K or \
+            t_ids.shape[:-1] != student_logits.shape[:-1] or t_logprobs.shape != t_ids.shape or \
+            t_logprobs.requires_grad or distill.transformed():
+        return plain(student_logits)[0].mean()
+    return distill.twice(student_logits, lambda z: (distill.kd_topk(z, t_ids.long(), t_logprobs),), plain)[0].mean()

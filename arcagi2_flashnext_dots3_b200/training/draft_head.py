@@ -18,7 +18,7 @@ Objective per start position q: alpha_k = sum_v min(q_k(v), p_k(v)), the probabi
 when drafts are sampled from q_k and verified against the target distribution p_k (the main model's next-token
 distribution at position q + k, renormalized over the hot vocabulary). E = sum_k prod_{j <= k} alpha_j is the
 expected number of accepted drafts. loss = -mean(E) + kl_weight * mean_k KL(p_k || q_k). alpha_k and
-the KL of a step come from :func:`..ops.distill.accept_kl`.
+the KL of a step come from :func:`..ops.distill.accept_kl` (:func:`_acceptance`).
 """
 from __future__ import annotations
 
@@ -97,6 +97,19 @@ class DraftHeadTrain(nn.Module):
             return {"dense": dense, "moe": self.inner.export_scales()[0]}
 
 
+def _acceptance(draft: torch.Tensor, target: torch.Tensor):
+    """(sum_v min(q, p), KL(p || q)) of every row of fp32 logits. The target's own gradient, derivatives other than backward's and
+    vocabularies beyond the kernels' limit go through torch operations."""
+    def plain(z):
+        lq, lp = torch.log_softmax(z, -1), torch.log_softmax(target, -1)
+        p = lp.exp()
+        return torch.minimum(lq.exp(), p).sum(-1), (p * (lp - lq)).sum(-1)
+
+    if target.requires_grad or draft.shape[-1] > distill.MAX_V or distill.transformed():
+        return plain(draft)
+    return distill.twice(draft, lambda z: distill.accept_kl(z, target), plain)
+
+
 def draft_objective(model: DraftHeadTrain, h_main: torch.Tensor, ids: torch.Tensor, target_logits: torch.Tensor,
                     K: int = 4, kl_weight: float = 0.3):
     """(loss, mean E) for one sequence. h_main [T, H]: the main model's final hidden states; ids [T] the tokens;
@@ -116,7 +129,7 @@ def draft_objective(model: DraftHeadTrain, h_main: torch.Tensor, ids: torch.Tens
     kl = x.new_zeros(())
     for k in range(1, K + 1):
         x = model.step(x, ids[k:k + Q], k - 1)
-        alpha, kl_k = distill.accept_kl(model.logits(x).float(), tl[k:k + Q])
+        alpha, kl_k = _acceptance(model.logits(x).float(), tl[k:k + Q])
         prod = prod * alpha
         E = E + prod
         kl = kl + kl_k.mean()

@@ -170,9 +170,9 @@ def seq_kd(model, path, chunk: int = 1024, grad: bool = True, w_tool: float = 1.
         rows = h.index_select(0, at - 1)
         w = torch.as_tensor(tool_weights(ids, pos, w_tool), device=dev)
         tlp_t = torch.as_tensor(tlp, device=dev)
-        if tid_t.shape[1] <= distill.MAX_K:
+        if tid_t.shape[1] <= distill.MAX_K and model.lm_head.shape[0] <= distill.MAX_V:
             loss, kl, first = VocabKD.apply(rows, model.lm_head, tid_t, tlp_t, w, max(1, chunk))
-        else:                                       # records of more tokens than the kernels list
+        else:                                       # more tokens than the kernels list
             lp_k = VocabTopK.apply(rows, model.lm_head, tid_t.clamp_min(0), max(1, chunk))
             kl = kl21(lp_k, tid_t, tlp_t)
             loss, kl, first = (kl * w).sum(), kl.detach(), lp_k.detach().argmax(1) == 0
