@@ -270,7 +270,8 @@ class SpecDecoder:
             raise ValueError("speculative sampling supports full-vocabulary temperature sampling (no top-k / top-p)")
         dev = llm.device
         drafts = self.drafter.propose(llm, seqs, k)
-        if self.use_graph and not (sampled and getattr(llm.model, "vocab_sharded", False)):
+        if self.use_graph and not (sampled and (getattr(llm.model, "vocab_sharded", False) or
+                                                not sampling.verifies(k, llm.cfg.vocab_size))):
             y, accepted = self._graph_step(seqs, drafts, sampled)
             return self._advance(seqs, drafts, y, accepted)
         ids = [[s.out[-1]] + list(d) for s, d in zip(seqs, drafts)]
@@ -309,7 +310,7 @@ class SpecDecoder:
             lg = m._mm(x, m.W["lm_head"], f8=False).float().view(len(seqs), k1, -1)
             return sharded_speculative_accept(lg, m.W["vocab_range"][0], dr, temps, seeds, steps, m.tp.group)
         lg = m.logits(x).view(len(seqs), k1, -1)
-        if lg.is_cuda:
+        if lg.is_cuda and sampling.verifies(self.k, lg.shape[-1]):
             t = [torch.tensor(v, dtype=ty).to(lg.device) for v, ty in
                  ((temps, torch.float32), (seeds, torch.int64), (steps, torch.int64))]
             acc, nxt = sampling.speculative_verify(lg, dr.to(lg.device), *t)

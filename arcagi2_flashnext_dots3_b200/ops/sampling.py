@@ -212,6 +212,11 @@ def speculative_accept(logits: torch.Tensor, drafts: torch.Tensor, temps, seeds,
     return acc, nxt
 
 
+def verifies(k: int, vocab: int) -> bool:
+    """Whether :func:`speculative_verify` takes k drafts over `vocab` tokens on the GPU (csrc/vocab.h kMaxK, kMaxV)."""
+    return k <= 128 and vocab <= 1 << 20
+
+
 def speculative_verify(logits: torch.Tensor, drafts: torch.Tensor, temps: torch.Tensor, seeds: torch.Tensor,
                        steps: torch.Tensor, draft_logits: torch.Tensor = None, n_draft: torch.Tensor = None):
     """:func:`speculative_accept` for whole batches on the device (csrc/k_vocab.cu), with nothing read by the host:
