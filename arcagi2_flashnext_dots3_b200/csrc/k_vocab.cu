@@ -537,8 +537,8 @@ __device__ __forceinline__ int load_id(const Teacher& t, int64_t i, int V) {
 constexpr int kCand = 512;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, int64_t ld, int64_t rows, int V, float kl,
-                                                              unsigned long long* parts, float* tops) {
+__global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, int64_t ld, int64_t rows, int V, int width,
+                                                              float kl, unsigned long long* parts, float* tops) {
   __shared__ unsigned long long warp_part[kWarps];
   const int tid = threadIdx.x;
   pdl_launch_dependents();
@@ -550,7 +550,8 @@ __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, i
   uint4 x[kUnit];
   load_unit(s, x);
   const float top = add_soft<T>(x, kl, m, soft);
-  tops[unit_index() * kThreads + tid] = isnan(soft.sum) ? INFINITY : top;     // a NaN (or +inf) among them: to be looked at
+  // a NaN (or +inf) among them: to be looked at
+  if (tid < width) tops[unit_index() * width + tid] = isnan(soft.sum) ? INFINITY : top;
 #pragma unroll
   for (int o = 16; o; o >>= 1) soft = join(soft, shfl_xor(soft, o));
   if ((tid & 31) == 0) warp_part[tid >> 5] = as_u64(soft.c, soft.sum);
@@ -562,8 +563,8 @@ __global__ void __launch_bounds__(kThreads) topk_units_kernel(const T* logits, i
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, int64_t ld, int V, int units, int k,
-                                                               int groups, float kl, const unsigned long long* parts,
+__global__ void __launch_bounds__(kThreads, 6) topk_select_kernel(const T* logits, int64_t ld, int V, int units, int width,
+                                                               int k, int groups, float kl, const unsigned long long* parts,
                                                                const float* tops, int32_t* ids, float* lp) {
   constexpr int N = Vec<T>::N;
   __shared__ unsigned long long cand[kCand], warp_key[kWarps];
@@ -572,13 +573,14 @@ __global__ void __launch_bounds__(kThreads) topk_select_kernel(const T* logits, 
   const int tid = threadIdx.x, shift = __ffs(kThreads / groups) - 1;
   const int64_t row = blockIdx.x;
   const Slice<T> s(logits + row * ld, V, V + N, 0);
-  tops += row * units * kThreads + tid;
+  tops += row * units * width + tid;
+  const int held = tid < width ? units : 0;        // rows of more than one unit have all threads' maxima
   pdl_wait();
   const auto each_top = [&](auto f) {              // f(unit, maximum) for this thread of every unit
-    for (int u0 = 0; u0 < units; u0 += 8) {
+    for (int u0 = 0; u0 < held; u0 += 8) {
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = u0 + i < units ? tops[(u0 + i) * kThreads] : -INFINITY;
+      for (int i = 0; i < 8; ++i) x[i] = u0 + i < held ? tops[(u0 + i) * kThreads] : -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) f(u0 + i, x[i]);
     }
@@ -1658,11 +1660,14 @@ int sm_count() {
   return n;
 }
 
-// Units per row of `z`: a row that starts off a 16-byte boundary may touch one vector more.
-int splits_of(Type type, Logits z, int64_t rows, int V, int vec = kUnit) {
+// Vectors per row of `z`, one more where a row may start off a 16-byte boundary, and units per row.
+int vectors_of(Type type, Logits z, int64_t rows, int V) {
   const int lanes = type == F32 ? 4 : 8;
   const bool aligned = (reinterpret_cast<uintptr_t>(z.p) & 15) == 0 && (rows == 1 || z.ld % lanes == 0);
-  return ((V + lanes - 1) / lanes + (aligned ? 0 : 1) + vec * kThreads - 1) / (vec * kThreads);
+  return (V + lanes - 1) / lanes + (aligned ? 0 : 1);
+}
+int splits_of(Type type, Logits z, int64_t rows, int V, int vec = kUnit) {
+  return (vectors_of(type, z, rows, V) + vec * kThreads - 1) / (vec * kThreads);
 }
 
 // Blocks per row (a cluster) and vectors of each tensor that a block keeps, in the kernels that look twice; `sides` tensors
@@ -1749,15 +1754,18 @@ struct Carver {
   }
 };
 struct TopWork {
+  int splits, width;           // units per row, maxima per unit: of the threads that have a vector
   unsigned long long* parts;
   float* tops;
   size_t bytes;
 };
-TopWork carve_topk(int64_t units, void* p) {
+TopWork carve_topk(Type type, Logits z, int64_t rows, int V, void* p) {
   Carver c{static_cast<char*>(p)};
   TopWork t{};
-  t.parts = c.take<unsigned long long>(units);
-  t.tops = c.take<float>(units * kThreads);
+  t.splits = splits_of(type, z, rows, V);
+  t.width = std::min(vectors_of(type, z, rows, V), kThreads);
+  t.parts = c.take<unsigned long long>(rows * t.splits);
+  t.tops = c.take<float>(rows * t.splits * t.width);
   t.bytes = c.used;
   return t;
 }
@@ -1775,24 +1783,23 @@ KdRows carve_kd(int64_t rows, int k, void* p, size_t& bytes) {
 }  // namespace
 
 size_t teacher_topk_workspace(Type type, Logits z, int64_t rows, int V) {
-  return carve_topk(rows * splits_of(type, z, rows, V), nullptr).bytes;
+  return carve_topk(type, z, rows, V, nullptr).bytes;
 }
 cudaError_t teacher_topk(Type type, Logits z, int64_t rows, int V, int k, float temp, int32_t* ids, float* lp,
                          void* workspace, cudaStream_t stream) {
-  const int splits = splits_of(type, z, rows, V);
-  const TopWork w = carve_topk(rows * splits, workspace);
+  const TopWork w = carve_topk(type, z, rows, V, workspace);
   const int groups = k <= 24 ? 32 : k <= 48 ? 64 : k <= 96 ? 128 : 256;
   const float kl = (float)(kLog2ed / temp);
   Shape units, select;
   units.blocks = select.blocks = rows;
-  units.units = splits;
+  units.units = w.splits;
   select.early = true;
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     const T* p = static_cast<const T*>(z.p);
-    const cudaError_t e = launch(topk_units_kernel<T>, units, stream, p, z.ld, rows, V, kl, w.parts, w.tops);
+    const cudaError_t e = launch(topk_units_kernel<T>, units, stream, p, z.ld, rows, V, w.width, kl, w.parts, w.tops);
     if (e != cudaSuccess) return e;
-    return launch(topk_select_kernel<T>, select, stream, p, z.ld, V, splits, k, groups, kl, w.parts, w.tops, ids, lp);
+    return launch(topk_select_kernel<T>, select, stream, p, z.ld, V, w.splits, w.width, k, groups, kl, w.parts, w.tops, ids, lp);
   });
 }
 
