@@ -59,13 +59,12 @@ constexpr int kUnit = 8;
 constexpr int kMaxCluster = 16;
 constexpr int kRowThreads = 256;     // of the kernels that look twice
 constexpr int kRowWarps = kRowThreads / 32;
-// Their blocks per SM and the vectors of each that shared memory keeps. One tensor: 40 KB in 48 registers (three to six
-// blocks are within 1%). Two tensors: 48 KB and 64 registers; five blocks spill (508 x 151936 bf16: 132 us instead of 118),
-// three are too few to cover the loads (2044 x 32768 fp32: 150 us instead of 136).
+// Their blocks per SM, and the vectors that a block keeps in shared memory (32 KB over its tensors). One tensor: five blocks of
+// 48 registers (three to six blocks are within 1%). Two tensors: four of 64 registers; five blocks spill (508 x 151936 bf16:
+// 132 us instead of 118), three are too few to cover the loads (2044 x 32768 fp32: 150 us instead of 136).
 constexpr int kRowBlocks = 5;
-constexpr int kRowKeep = 2560;
 constexpr int kPairBlocks = 4;
-constexpr int kPairKeep = 3072;
+constexpr int kKeep = 2048;
 constexpr float kTailFloor = 1e-8f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLog2ed = 1.4426950408889634;
@@ -1672,7 +1671,7 @@ int splits_of(Type type, Logits z, int64_t rows, int V, int vec = kUnit) {
 
 // Blocks per row (a cluster) and vectors of each tensor that a block keeps, in the kernels that look twice; `sides` tensors
 // share a block. A cluster costs its barriers, so it grows only
-//   * until what all running blocks do not keep takes half of L2, as the second look reads it there (clusters of 1, 2, 4, 8,
+//   * until what all running blocks do not keep takes 72 MB of L2's 126, as the second look reads it there (clusters of 1, 2, 4, 8,
 //     16: 1024 x 151936 fp32 with gradient 340, 300, 286, 250, 329 us, taken 8; 2048 x 152064 bf16 312, 283, 271, 353,
 //     547 us, taken 4; acceptance of 2044 x 32768 fp32 159, 136, 167, 240, 479 us, taken 2);
 //   * until one wave of blocks fills the GPU, as long as each thread has a vector (acceptance of 4 x 151936 bf16 46, 27, 18,
@@ -1681,20 +1680,13 @@ struct Plan {
   int cluster, keep, smem;
 };
 Plan plan_of(Type type, int64_t rows, int V, int sides) {
-  const int total = V / (type == F32 ? 4 : 8) + 1, held = sides == 1 ? kRowKeep : kPairKeep;
+  const int total = V / (type == F32 ? 4 : 8) + 1;
   const int64_t slots = (sides == 1 ? kRowBlocks : kPairBlocks) * sm_count();
   int c = 1;
-  while (c < kMaxCluster && (total * sides / c - held) * 16ll * slots > 64 << 20) c *= 2;
+  while (c < kMaxCluster && (total * sides / c - kKeep) * 16ll * slots > 72 << 20) c *= 2;
   while (c < kMaxCluster && total * sides > kRowThreads * c && rows * c * 2 <= slots) c *= 2;
-  const int per = (total + c - 1) / c, keep = std::min(per, held / sides) / kRound * kRound;
+  const int per = (total + c - 1) / c, keep = std::min(per, kKeep / sides) / kRound * kRound;
   return {c, keep, keep * sides * 16};
-}
-
-cudaError_t allow(const void* f, int cluster, size_t smem) {
-  cudaError_t e = cudaSuccess;
-  if (smem > 32768) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  return e;
 }
 
 struct Shape {
@@ -1706,8 +1698,10 @@ struct Shape {
 };
 template <typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), const Shape& s, cudaStream_t stream, A... args) {
-  cudaError_t e = allow(reinterpret_cast<const void*>(kernel), s.cluster, s.smem);
-  if (e != cudaSuccess) return e;
+  if (s.cluster > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
   if (s.blocks < 1 || s.blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)s.blocks);
