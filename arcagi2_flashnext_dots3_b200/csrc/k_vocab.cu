@@ -34,10 +34,12 @@
 //     (cp.async, read back only by the thread that copied it) and streams the rest, once for each look: the second time it
 //     comes from L2. Nothing is exchanged outside a cluster, whose blocks write their parts into each other's shared
 //     memory and finish the row's statistics each by itself, in rank order. One kernel over both looks without clusters,
-//     its blocks waiting for the other blocks of their row through global memory, took 276 us where this takes 238
+//     its blocks waiting for the other blocks of their row through global memory, took 276 us where this takes 239
 //     (1024 x 151936 fp32), and a loss kernel followed by a gradient kernel 287;
 //   * exp(x) is ex2(x log2 e / T - c) with c = m log2 e / T rounded once and used for the sum and for every
-//     probability alike, so that rounding cancels; one FMA and one ex2 per element.
+//     probability alike, so that rounding cancels; one FMA and one ex2 per element. The offset's rounding stays in range
+//     while |z| / T is below 2^30, logits of 1000 at the smallest T (1e-6); verification, whose temperatures come with requests,
+//     takes the largest logit off instead.
 // Times below are of one B200, GPU time per call with inputs larger than L2, and "of the copy rate" is of 6551 GB/s.
 #include <algorithm>
 #include <cstdint>
@@ -530,9 +532,12 @@ __device__ __forceinline__ int load_id(const Teacher& t, int64_t i, int V) {
 // that at least k values reach and few others do (with k = 20 of 32 groups about 31 of independent values). The vectors
 // of threads whose maximum reaches it are read again, one per thread; what reaches it is collected and ranked by counting.
 // More than kCand (long runs of equal logits): k rounds of the smallest key above the last, which any input ends in.
-// Bound by memory: 103 us for 1024 x 151936 fp32 (93% of the copy rate), 138 us for 2048 x 152064 bf16 (69%: twice the ex2 per
-// byte). Few rows: 12 us for 8 x 151936 fp32, the two kernels' latencies. Selecting in each unit, and joining lists, took
-// 133 and 317 us: the selection's barriers then stand between a block's loads and the next block's.
+// 104 us for 1024 x 151936 fp32 (91% of the copy rate), 119 us for 2048 x 152064 bf16 (80%): the first kernel reads at 106% and 93%
+// of the copy rate (89 and 102 us), and the selection of the last rows runs behind it (18 and 23 us by itself). Few rows: 12 us for
+// 8 x 151936 fp32, the two kernels' latencies. Selecting in each unit, and joining lists, took 133 and 317 us: the selection's
+// barriers then stand between a block's loads and the next block's.
+// The selection is held to six blocks per SM: with the registers it takes by itself (47) 2048 rows took 121 us; eight blocks
+// spill, 117 us there and 13.8 instead of 12.0 at 8 rows.
 constexpr int kCand = 512;
 
 template <typename T>
@@ -798,8 +803,8 @@ __device__ __forceinline__ float kd_loss(const TeacherSums& e, const Soft& tail)
   if (e.mass != 0.0) l += e.mass * kLn2d * ((double)c - e.c + log2(total));
   return (float)l;
 }
-// The gradient at a teacher's token is w (c_k - ps sum c) = w (pull ps - pt) with pull = tt / ts - sum c = tt / ts (1 - sum ps) + sum
-// pt, that is tt + sum pt, without tt at the floor. Formed as the difference it loses the tail of a sure student (ts = 1e-6: 0.06
+// The gradient at a teacher's token is w (c_k - ps sum c) = w (pull ps - pt) with pull = tt / ts - sum c = tt / ts (1 - sum ps) +
+// sum pt, that is tt + sum pt, without tt at the floor. Formed as the difference it loses the tail of a sure student (ts = 1e-6: 0.06
 // of a gradient of 0.3).
 __device__ __forceinline__ float pull_of(const TeacherSums& e, float ratio) {
   return (float)e.mass + (ratio > 0.f ? e.tt : 0.f);
@@ -940,7 +945,7 @@ struct ShareIds {
 
 // Loss and gradient of a row by one block or cluster. The owner of a teacher's token takes it out (-inf) before the first
 // look, which so sums the tail alone (a confident student's tail is lost in 1 - sum ps); after the second look it writes
-// the token's gradient. 238 us for 1024 x 151936 fp32 (80% of the copy rate for one read and one write), 522 us for 4096 x
+// the token's gradient. 239 us for 1024 x 151936 fp32 (80% of the copy rate for one read and one write), 521 us for 4096 x
 // 152064 bf16 (73%). A block's phases (load, reduce, write) leave its share of the memory idle between them, which only the
 // other blocks of the SM fill; in bf16 the two ex2 per 4 bytes take 60% of the time as well.
 template <typename T>
@@ -1197,7 +1202,7 @@ __device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&
 
 // One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p) and of q h. 138 us for 2044
 // x 32768 fp32 (59% of the copy rate), 122 us for 508 x 151936 bf16 (39%): three ex2 per pair of logits (64 us of the 122) and
-// some 34 instructions come near the time of the loads, and the two looks of a block do not overlap. h by comparisons, with the
+// 33 instructions come near the time of the loads, and the two looks of a block do not overlap. h by comparisons, with the
 // few equal tokens in a branch, took 143 and 129 us; with the mass of q on either side summed by itself (a fourth ex2) 144 and 133.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const T* draft, int64_t ldq, const T* target,
@@ -1311,7 +1316,7 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
   stats[row] = nothing ? AcceptRow{} : AcceptRow{rq, fq, rp, fp, steep, middle, fq * w.y};
 }
 
-// The gradient from the row's statistics, elementwise. 117 us for 2044 x 32768 fp32 (105% of the copy rate), 70 us for 508 x
+// The gradient from the row's statistics, elementwise. 119 us for 2044 x 32768 fp32 (103% of the copy rate), 70 us for 508 x
 // 151936 bf16 (101%).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, int64_t ldq, const T* target, int64_t ldp,
@@ -1353,16 +1358,16 @@ __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, in
 // parts, finds the first rejected draft and draws from that position alone: the race costs a hash per token and is run for
 // one row of the k + 1. A draw needs -log(u) / r below the best so far; -log(u) >= 1 - u, which is the hash's integer, so
 // the logarithm and the division are taken for the few tokens that can win.
-// 55.5 us for 64 sequences of 3 soft drafts x 151936 bf16: 31 us the rows (68% of the copy rate), 24 us the draw, bound by the 50
+// 55.5 us for 64 sequences of 3 soft drafts x 151936 bf16: 31 us the rows (68% of the copy rate), 24 us the draw, bound by the 51
 // instructions per token, most of them the hash's 64-bit products. 34.9 us for 32 sequences of up to 7 point-mass drafts x
 // 152064 fp32 (68% of the copy rate over both). One sequence of 3: 10 us, latency.
 constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr int kDrawVec = 2;          // vectors that a thread requests at once
 
-// Temperatures come with requests, from next to nothing to infinity. kl stays finite; at T = 1e20 all logits weigh the same to fp32,
-// and a masked one still nothing. An offset m kl rounded once would be off by more than 2^127 from a T of some 1e-7 down, so
-// here the largest logit is taken off first and the rest scaled: one more operation per logit (54.0 -> 55.5 us for 64 sequences
+// Temperatures come with requests, from next to nothing to infinity. kl stays finite; at T = 1e20 all logits weigh the same to
+// fp32, and a masked one still nothing. The rounding of an offset m kl leaves fp32's range of exponents where |z| / T passes 2^30,
+// so here the largest logit is taken off first and the rest scaled: one more operation per logit (54.0 -> 55.5 us for 64 sequences
 // of 3 soft drafts x 151936 bf16).
 __device__ __forceinline__ float scale_of(float temp) { return fminf(kLog2e / fminf(temp, 1e20f), 3e38f); }
 // sum = sum over elements of 2^((z - m) kl), m the largest z or kFloor

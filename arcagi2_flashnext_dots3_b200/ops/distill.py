@@ -11,8 +11,9 @@ flashnext/training/draft_head/train.py); its code works in torch on whole [rows,
 
 Logits are [rows, vocab] in fp32, fp16 or bf16 (vocab up to 2^20; rows may be strided). A logit at or below -1e30
 (-inf, the lowest fp32 / bf16 value) is masked and has probability 0; a row with nothing left gives loss 0, gradient
-0 and id -1. A NaN makes its row's results NaN. Results per row are fp32, gradients have the logits' type. Nothing
-here reads from the host, so every call can be captured in a CUDA graph.
+0 and id -1. A NaN makes its row's results NaN. Temperatures are 1e-6 to 1e6, and logits on the GPU at most 2^30 T.
+Results per row are fp32, gradients have the logits' type. Nothing here reads from the host, so every call can be
+captured in a CUDA graph.
 """
 from __future__ import annotations
 
@@ -237,7 +238,8 @@ def accept_kl(draft: torch.Tensor, target: torch.Tensor, temperature: float = 1.
     """(alpha, kl) fp32 [rows] of draft logits against target logits of the same shape and type: alpha = sum_v
     min(q_v, p_v), the probability that speculative verification accepts a token drawn from q, and kl = KL(p || q),
     with q, p the softmaxes at `temperature`. Differentiable in the draft; the target is taken as given. Where q_v =
-    p_v (for the kernels: to within a few fp32 roundings) the gradient of alpha is the mean of its two sides. A row in which either side has no token left gives zeros."""
+    p_v (for the kernels: to within a few fp32 roundings) the gradient of alpha is the mean of its two sides. A row in
+    which either side has no token left gives zeros."""
     if draft.is_cuda:
         return native.C().accept_kl(draft, target, temperature)
     draft = _rows(draft, "draft logits")

@@ -229,11 +229,12 @@ def speculative_verify(logits: torch.Tensor, drafts: torch.Tensor, temps: torch.
     noise of (seed, step + j, token) they would otherwise share. ``n_draft`` int32 [B]: drafts of each sequence, 0 to
     k; later positions are not read.
 
-    Any temperature goes: the largest logit is taken off before the division, so a T next to 0 keeps the largest logits alone,
-    and beyond 1e20 all unmasked tokens weigh the same. T <= 0 is greedy: accepted while the draft is the argmax (lowest id on ties), which is also the next token. A draft
-    outside the vocabulary is rejected. Masked logits (at or below -1e30) are never drawn; a residual that is empty in
-    fp32 draws from p. A position with no token left, or with a NaN among its logits, rejects its draft and gives -1; a row of
-    draft_logits with a NaN is no distribution: its draft is rejected and the next token comes from p."""
+    Any temperature goes: the largest logit is taken off before the division, so a T next to 0 leaves the largest logits
+    alone, and beyond 1e20 all unmasked tokens weigh the same. T <= 0 is greedy: accepted while the draft is the argmax
+    (lowest id on ties), which is also the next token. A draft outside the vocabulary is rejected. Masked logits (at or
+    below -1e30) are never drawn; a residual that is empty in fp32 draws from p. A position with no token left, or with a
+    NaN among its logits, rejects its draft and gives -1; a row of draft_logits with a NaN is no distribution: its draft is
+    rejected and the next token comes from p."""
     if logits.is_cuda:
         return native.C().spec_verify(logits, drafts, temps, seeds, steps, draft_logits, n_draft)
     if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
