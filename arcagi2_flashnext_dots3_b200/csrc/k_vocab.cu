@@ -1200,9 +1200,9 @@ __device__ __forceinline__ void add_pair(const uint4 (&xq)[kVec], const uint4 (&
   a.d += sum(d);
 }
 
-// One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p) and of q h. 138 us for 2044
-// x 32768 fp32 (59% of the copy rate), 122 us for 508 x 151936 bf16 (39%): three ex2 per pair of logits (64 us of the 122) and
-// 33 instructions come near the time of the loads, and the two looks of a block do not overlap. h by comparisons, with the
+// One row by one block or cluster. First look: both softmaxes and d; second look: the sums of min(q, p) and of q h. 137 us for 2044
+// x 32768 fp32 (60% of the copy rate), 123 us for 508 x 151936 bf16 (38%): three ex2 per pair of logits (64 us of the 123) and
+// some 34 instructions come near the time of the loads, and the two looks of a block do not overlap. h by comparisons, with the
 // few equal tokens in a branch, took 143 and 129 us; with the mass of q on either side summed by itself (a fourth ex2) 144 and 133.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const T* draft, int64_t ldq, const T* target,
@@ -1266,7 +1266,8 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
   const float per_tie = 0x1p20f / (1.f + fabsf(gap));
   const float steep = -kl * per_tie, middle = fmaf(gap, per_tie, 0.5f);
   Two least = two(0.f), held = two(0.f);     // sums of min(q, p), and of it times h: sum q h, as h = 0 where q > p
-  const Two k2 = two(kl), bq = two(-rq), bp = two(-rp);
+  // rq and rp are rounded: what they lose differs, and is given back to q before the two are compared
+  const Two k2 = two(kl), bq = two(-rq), bp = two(-rp), to_p = two((rq - rp) - gap);
   const auto look = [&](const uint4& uq, const uint4& up) {
     float q[N], p[N];
     Vec<T>::unpack(uq, q);
@@ -1274,7 +1275,8 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
       const Two zq = two(q[k], q[k + 1]), zp = two(p[k], p[k + 1]);
-      const float2 eq = halves(fma2(zq, k2, bq)), ep = halves(fma2(zp, k2, bp)), h = share2(zq, zp, steep, middle);
+      const float2 eq = halves(add2(fma2(zq, k2, bq), to_p)), ep = halves(fma2(zp, k2, bp));
+      const float2 h = share2(zq, zp, steep, middle);
       const Two e = two(ex2(fminf(eq.x, ep.x)), ex2(fminf(eq.y, ep.y)));
       least = add2(least, e);
       held = fma2(e, two(h.x, h.y), held);
@@ -1310,13 +1312,13 @@ __global__ void __launch_bounds__(kRowThreads, kPairBlocks) accept_kernel(const 
   const float fq = exp2f((float)((double)rq - (cq + lq))), fp = exp2f((float)((double)rp - (cp + lp)));
   const bool nothing = a.sq == 0.f || a.sp == 0.f;
   const bool nan = isnan(a.sq) || isnan(a.sp);            // the minimum drops a NaN operand
-  alpha[row] = nothing ? 0.f : nan ? NAN : fp * w.x + (fq - fp) * w.y;
+  alpha[row] = nothing ? 0.f : nan ? NAN : fp * w.x;
   out_kl[row] = nothing ? 0.f : (float)(kLn2d * ((double)a.d / a.sp + lq - lp));
   if (!stats) return;
-  stats[row] = nothing ? AcceptRow{} : AcceptRow{rq, fq, rp, fp, steep, middle, fq * w.y};
+  stats[row] = nothing ? AcceptRow{} : AcceptRow{rq, fq, rp, fp, steep, middle, fp * w.y};
 }
 
-// The gradient from the row's statistics, elementwise. 119 us for 2044 x 32768 fp32 (103% of the copy rate), 70 us for 508 x
+// The gradient from the row's statistics, elementwise. 118 us for 2044 x 32768 fp32 (104% of the copy rate), 69 us for 508 x
 // 151936 bf16 (101%).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) accept_bwd_kernel(const T* draft, int64_t ldq, const T* target, int64_t ldp,

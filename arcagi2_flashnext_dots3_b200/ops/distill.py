@@ -57,9 +57,9 @@ def _temperature(t: float) -> float:
     return t
 
 
-def _log_softmax(x: torch.Tensor, t: float) -> torch.Tensor:
-    """log softmax(x / t) in fp32 with masked logits at -inf; a row with nothing left is -inf throughout."""
-    z = x.float()
+def _log_softmax(x: torch.Tensor, t: float, dtype=torch.float32) -> torch.Tensor:
+    """log softmax(x / t) with masked logits at -inf; a row with nothing left is -inf throughout."""
+    z = x.to(dtype)
     z = z.masked_fill(z <= MASKED, float("-inf")) / t
     nothing = (z == float("-inf")).all(-1, keepdim=True)
     return torch.log_softmax(z.masked_fill(nothing, 0.0), -1).masked_fill(nothing, float("-inf"))
@@ -207,13 +207,13 @@ def kd_topk_grad(logits: torch.Tensor, t_ids: torch.Tensor, t_lp: torch.Tensor, 
 def _accept_cpu(draft, target, t, g_alpha=None, g_kl=None):
     """(alpha, kl) per row, or with their gradients the gradient of the draft."""
     ninf = float("-inf")
-    lq, lp = _log_softmax(draft, t), _log_softmax(target, t)
+    lq, lp = (_log_softmax(x, t, torch.float64) for x in (draft, target))
     nothing = (lq == ninf).all(-1) | (lp == ninf).all(-1)
     q, p = lq.exp(), lp.exp()
     if g_alpha is None:
         kl = torch.where(p > 0, p * (lp - lq), 0.0)
         kl = torch.where(torch.isnan(p), p, kl).sum(-1)
-        return torch.where(nothing, 0.0, torch.minimum(q, p).sum(-1)), torch.where(nothing, 0.0, kl)
+        return torch.where(nothing, 0.0, torch.minimum(q, p).sum(-1)).float(), torch.where(nothing, 0.0, kl).float()
     # h - A of a token from the masses of the other sides: a sure token's 1 - A is lost in a difference
     below, even, above = ((q * on).sum(-1, keepdim=True) for on in (lq < lp, lq == lp, lq > lp))
     h_a = torch.where(lq < lp, above + 0.5 * even, torch.where(lq == lp, 0.5 * (above - below), -(below + 0.5 * even)))

@@ -120,3 +120,23 @@ def test_training_and_evaluation_give_one_alpha():
         a, k = distill.accept_kl(q, p)
         b, l = distill.accept_kl(q.clone().requires_grad_(), p)
         assert torch.equal(a, b.detach()) and torch.equal(k, l.detach())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shift", [0.0, 100.0, -1000.0])
+def test_alpha_keeps_its_digits(shift, device):
+    """alpha of sure and of flat rows, whatever constant the logits carry: each probability is an exponential of z - max, so
+    alpha is off by the rounding of the exponentials' arguments, at most 2^-20 for arguments below 16, of the instruction (2
+    ulp) and of the sums: 2^-18 of itself covers them. (Smaller probabilities have a larger relative error and no weight.)"""
+    g = torch.Generator().manual_seed(6)
+    for V in (2, 300, 32768, 50001):
+        n = 60
+        top = torch.randint(0, V, (n,), generator=g)
+        miss = torch.exp(torch.rand(2, n, generator=g) * -18)
+        q, p = (sure(g, n, V, miss[i].clamp_max(0.9), top) + shift for i in (0, 1))
+        q[::4] = torch.randn(15, V, generator=g) + shift
+        p[::4] = q[::4] + 0.5 * torch.randn(15, V, generator=g)
+        q[1::4] = p[1::4] + 0.001 * torch.randn(15, V, generator=g)
+        a, _ = distill.accept_kl(q.to(device), p.to(device))
+        want = torch.minimum(torch.log_softmax(q.double(), -1), torch.log_softmax(p.double(), -1)).exp().sum(-1)
+        assert float((a.cpu().double() - want).abs().div(want).max()) <= 2.0 ** -18
