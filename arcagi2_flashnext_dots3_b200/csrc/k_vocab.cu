@@ -804,8 +804,8 @@ __device__ __forceinline__ float kd_loss(const TeacherSums& e, const Soft& tail)
   return (float)l;
 }
 // The gradient at a teacher's token is w (c_k - ps sum c) = w (pull ps - pt) with pull = tt / ts - sum c = tt / ts (1 - sum ps) +
-// sum pt, that is tt + sum pt, without tt at the floor. Formed as the difference it loses the tail of a sure student (ts = 1e-6: 0.06
-// of a gradient of 0.3).
+// sum pt, that is tt + sum pt, without tt at the floor. Formed as the difference it loses the tail of a sure student (ts = 1e-6:
+// 0.06 of a gradient of 0.3).
 __device__ __forceinline__ float pull_of(const TeacherSums& e, float ratio) {
   return (float)e.mass + (ratio > 0.f ? e.tt : 0.f);
 }

@@ -162,7 +162,8 @@ class SpecGraph:
         m.commit(acc + 1)
         self.y.copy_(y)
         self.acc.copy_(acc)
-        y = y.clamp_min(0)
+        if self.sampled:
+            y = y.clamp_min(0)
         if self.head is not None:
             h = self.head
             xm = h.step(x, y.reshape(-1), self.slots, self.pos, k1)
